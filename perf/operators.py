@@ -202,6 +202,7 @@ def prepare(case, seed):
         s["w"] = _pack4((torch.randn(case["n"], case["k"], device="cuda", generator=g) * 0.02).to(torch.bfloat16).float())
         if own:
             s["M"] = M = _lib()
+            s["weight"] = M.Mxfp4Weights([(*s["w"], case["n"], case["k"])])
             s["y"] = torch.empty(case["rows"], case["n"], dtype=DT[case["dtype"]], device="cuda")
             s["work"] = torch.empty(M.linear_mxfp4_work_bytes(case["rows"], case["k"]), dtype=torch.uint8, device="cuda")
     elif op == "experts":
@@ -210,8 +211,8 @@ def prepare(case, seed):
             s["M"] = M = _lib()
             s["moe"] = M.MoE(case["rows"], case["dim"], case["experts"], case["topk"], hidden=case["hidden"],
                              router_dtype=M.F32 if case["router"] == "f32" else M.BF16, training=False)
-            s["wup"] = [(c, sc, case["hidden"], case["dim"]) for c, sc in s["w"][0]]
-            s["wdown"] = [(c, sc, case["dim"], case["hidden"]) for c, sc in s["w"][1]]
+            s["wup"] = M.Mxfp4Weights([(c, sc, case["hidden"], case["dim"]) for c, sc in s["w"][0]])
+            s["wdown"] = M.Mxfp4Weights([(c, sc, case["dim"], case["hidden"]) for c, sc in s["w"][1]])
             s["y"] = torch.empty_like(s["x"])
     else:
         x, s["gamma"], g = _ln_inputs(case, seed)
@@ -257,7 +258,7 @@ def _run_own(s):
             M.act8_restore(s["codes"], s["scales"], s["y"], fmt)
         return s["y"]
     if op == "linear":
-        M.linear_mxfp4(s["x"], (*s["w"], c["n"], c["k"]), s["y"], s["work"])
+        M.linear_mxfp4(s["x"], s["weight"], s["y"], s["work"])
         return s["y"]
     if op == "experts":
         s["moe"].forward_mxfp4(s["x"], s["wr"], s["wup"], s["wdown"], s["y"])
