@@ -1,0 +1,83 @@
+/* C ABI of the microscaled operators around the MoE block on B200 (sm_100a): 4-bit matrices and their products, and
+ * 8-bit checkpoints of activations.
+ *
+ * A block is 32 neighbouring elements of a row. It keeps 32 element codes and one scale byte b:
+ *     value_i = code_i * 2^(b - 127),    b = 255: the block held an infinity or a NaN; all its values are NaN.
+ * The scale is the smallest power of two (not below 2^-127) at which no element of the block passes the element type's
+ * largest value; the elements are x / scale rounded to nearest, ties to even. Nothing saturates, and no input is refused
+ * for its values.
+ *     e2m1 (largest 6)      MXFP4, 4.25 bits per element: weights and activations of a product
+ *     e4m3 (448), e5m2 (57344)   8.25 bits per element: what a backward pass keeps of an activation ("act8")
+ *
+ * 4-bit matrix (rows, cols), cols a multiple of 64: `codes` rows * cols / 2 bytes, row-major, element 2i of a row in the low
+ * half of its byte i; `scales` tmt_moe_mxfp4_scale_bytes(rows, cols) bytes in the order the tensor cores read them:
+ * tiles of 128 rows x 4 blocks, 512 bytes each, the tiles of a 128-row band one after the other; within a tile the byte
+ * of (row, block) is (row % 32) * 16 + (row % 128 / 32) * 4 + block % 4. Bytes of rows past the last are never used.
+ * 8-bit matrix (rows, cols), cols a multiple of 32: `codes` rows * cols bytes, `scales` rows * cols / 32 bytes, both row-major.
+ *
+ * Conventions as in tmt_moe.h and tmt_norm.h: 0 / -1, message from tmt_moe_last_error(), device pointers, 16-byte aligned
+ * (what cudaMalloc returns is), nothing allocates, nothing synchronises, nothing calls exit(). Work is queued on `stream`
+ * of the current device; a tensor that lies on another device, or in host memory that the device cannot read, is refused.
+ * Calls may run side by side on several streams (they share no state), and may be captured into a graph. rows = 0 is
+ * allowed where no handle is involved and does nothing. */
+#ifndef TMT_MX_H
+#define TMT_MX_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "tmt_moe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Formats of the 8-bit checkpoints. */
+enum { TMT_ACT8_OFF = 0, TMT_ACT8_E4M3 = 1, TMT_ACT8_E5M2 = 2 };
+
+/* A 4-bit weight matrix W (rows = outputs, cols = inputs), [out,in] as everywhere in tmt_moe.h. */
+typedef struct tmt_mxfp4_weight {
+    const void* codes;
+    const void* scales;
+    int rows, cols;
+} tmt_mxfp4_weight;
+
+/* Bytes of the scale buffer of a 4-bit (rows, cols) matrix; 0 for a shape that is not supported. */
+size_t tmt_moe_mxfp4_scale_bytes(long long rows, int cols);
+
+/* X (rows, cols), dtype TMT_MOE_BF16 or TMT_MOE_F32 -> 4-bit blocks. cols: a multiple of 64. One matrix per call: a list of
+ * experts' matrices is quantised one by one, each into a buffer of its own. */
+int tmt_moe_quantize_mxfp4(const void* X, int dtype, long long rows, int cols, void* codes, void* scales, void* stream);
+/* 4-bit blocks -> Y (rows, cols), exact in both dtypes (bf16: but for values below its smallest normal number). */
+int tmt_moe_dequantize_mxfp4(const void* codes, const void* scales, long long rows, int cols, void* Y, int dtype, void* stream);
+
+/* Y = A W^T with both operands in 4-bit blocks, on the block-scaled tensor-core instruction: products exact, sums in fp32,
+ * rounded once to `dtype`. A (rows, W->cols), Y (rows, W->rows) row-major and dense; W->rows: a multiple of 8, W->cols: a
+ * multiple of 64. status (device int, may be NULL): receives a code of tmt_moe_device_status when a bounded wait ran out;
+ * never cleared here. */
+int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, const tmt_mxfp4_weight* W, void* Y, int dtype,
+                         int* status, void* stream);
+
+/* A dense layer: X (rows, W->cols) bf16 or fp32 is quantised into `work` (tmt_moe_linear_mxfp4_work_bytes bytes, contents
+ * before and after the call do not matter) and multiplied. Two calls that may run at the same time need a work buffer each. */
+size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols);
+int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
+                         size_t work_bytes, int* status, void* stream);
+
+/* tmt_moe_forward with both expert products on 4-bit blocks (hidden > 0, training = 0, a single rank). The router, the
+ * gate weights, the statistics and the residual (beta) are those of tmt_moe_forward, bit for bit; a token's row is quantised
+ * on its way into its experts' groups; P = q4(X) Wup^T, then q4(silu(P)) straight from the fp32 accumulators, then
+ * gate * (q4(silu(P)) Wdown^T). Wup / Wdown: HOST arrays of E descriptors whose device memory must stay valid while the
+ * handle uses them. The first call on a handle allocates its buffers, and a call with other pointers than the last one
+ * uploads a table: both outside any stream capture. */
+int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
+                          const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
+
+/* 8-bit checkpoint of an activation X (rows, cols), and back. format: TMT_ACT8_E4M3 or TMT_ACT8_E5M2; cols: a multiple of 32. */
+int tmt_moe_act8_save(const void* X, int dtype, long long rows, int cols, int format, void* codes, void* scales, void* stream);
+int tmt_moe_act8_restore(const void* codes, const void* scales, long long rows, int cols, int format, void* Y, int dtype, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

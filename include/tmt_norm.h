@@ -40,6 +40,27 @@ size_t tmt_ln_backward_scratch_bytes(int rows, int dim);
 int tmt_ln_backward(const void* X, const void* dY, const float* gamma, const float* mean, const float* rstd, void* dX,
                     float* dGamma, float* dBeta, int rows, int dim, void* scratch, void* stream);
 
+/* ---- with an 8-bit checkpoint of the input (formats and layout: include/tmt_mx.h; no counterpart in the reference, which
+ * keeps a bf16 copy of every layer's input for layernorm_bwd, model.cu:509-511) ----
+ * What the backward pass needs of X is kept in 8.25 bits per element: rows * dim code bytes and rows * dim / 32 scale bytes.
+ * dim: a multiple of 32, at most 8192; format: TMT_ACT8_E4M3 (1) or TMT_ACT8_E5M2 (2). Tensors as in tmt_mx.h (16-byte aligned,
+ * on the current device); mean, rstd, dGamma, dBeta and, in the backward pass, gamma need 4-byte alignment alone. */
+
+/* tmt_ln_forward (the same bits in Y, mean and rstd), and the checkpoint of X in the same pass over it. rows = 0 does nothing. */
+int tmt_ln_forward_act8(const void* X, const float* gamma, const float* beta, void* Y, float* mean, float* rstd, void* codes,
+                        void* scales, int format, int rows, int dim, void* stream);
+
+/* Bytes of device scratch tmt_ln_backward_act8 needs for this shape; 0 for a shape that is not supported. Contents before and
+ * after the call do not matter; two calls that may run at the same time need a scratch each. */
+size_t tmt_ln_backward_act8_scratch_bytes(int rows, int dim);
+
+/* The gradient of the LayerNorm with x replaced by the checkpoint's value, and mean and rstd those of the forward pass:
+ * xh = (x - mean) * rstd, g = dY * gamma, dX = rstd * (g - sum(g) / dim - xh * (sum(g * xh) / dim)), dGamma = sum over the rows
+ * of dY * xh, dBeta = sum of dY. Sums in fp32, in an order fixed by the shape; dX is rounded once to bf16; dGamma and dBeta
+ * are written. A NaN block of the checkpoint gives NaN in its row of dX and in its columns of dGamma. */
+int tmt_ln_backward_act8(const void* codes, const void* scales, int format, const void* dY, const float* gamma, const float* mean,
+                         const float* rstd, void* dX, float* dGamma, float* dBeta, int rows, int dim, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,15 @@ struct Profiler {
     double ms[kNumPhases] = {0};
     long long count[kNumPhases] = {0};
 };
+// Buffers of tmt_moe_forward_mxfp4 (mx_moe.cu), allocated at its first call: the grouped rows and their SiLU outputs as 4-bit
+// blocks, and the per-expert tables of the weights last handed in.
+struct MxState {
+    uint8_t *x_codes = nullptr, *x_scales = nullptr, *h_codes = nullptr, *h_scales = nullptr;
+    CUtensorMap x_map[2] = {}, h_map[2] = {};      // [0] many-row form, [1] few-row form
+    CUtensorMap* tables = nullptr;                 // [2][E] weight maps: up, down
+    const uint8_t** scale_tab = nullptr;           // [2][E]
+    std::vector<const void*> key;                  // the pointers the tables were built from
+};
 }  // namespace tmt
 
 constexpr int kGemmCycLaunches = 16;   // GEMM launches whose cycle counters are kept (a ring)
@@ -95,6 +104,7 @@ struct tmt_moe {
     // call in progress, the normalised rows, and the statistics of the stand-alone kernel for larger batches
     const float* ln_gamma = nullptr; const float* ln_beta = nullptr;
     uint16_t* xn = nullptr; float* ln_stats = nullptr;
+    tmt::MxState mx;
     // expert parallelism
     tmt_ep_state* ep = nullptr;
     int* ep_world_counts = nullptr;

@@ -1,0 +1,447 @@
+// Products of 4-bit microscaled matrices on the block-scaled tensor-core instruction of sm_100a
+// (tcgen05.mma kind::mxf4, e2m1 operands, one e8m0 scale per 32 elements of each operand).
+//
+//   acc[i, j] = sum over blocks b of  sP[i, b] sQ[j, b]  sum over the block of qP qQ
+//
+// P is the operand on the 128-row side of the MMA, Q the one on its column side. Many rows: P = activations, Q = weights.
+// Few rows (a decode step): P = weights, Q = activations, so that a tile is 128 weight rows x the rows there are (in steps of 32,
+// up to 128) instead of 128 mostly empty rows, and the call is bound by streaming the weights once.
+//
+// Codes travel by TMA in boxes of 128 bytes (256 elements of k) with the 128-byte swizzle, exactly as a bf16 operand of 64
+// elements would; an MMA takes 64 elements (32 bytes). Scales travel as whole 512-byte tiles (128 rows x 4 blocks) by untiled
+// bulk copies into shared memory and from there by tcgen05.cp (32 lanes x 16 bytes, repeated for the four lane quarters) into
+// tensor memory, 4 columns per tile; the MMA reads two of the four blocks, picked by the scale ids of its descriptor. An MMA and
+// the copies issued before it by the same thread run in order, so the scale columns need no second buffer.
+//
+// Warps: 0 = TMA producer of P, 1 = MMA issuer and TMEM owner, 2..5 = epilogue, 6 = TMA producer of Q. Persistent over tiles,
+// two accumulators in tensor memory. Every wait is bounded, as in the bf16 kernels.
+#include <stdexcept>
+#include <string>
+
+#include "launch_pdl.cuh"
+#include "mx.cuh"
+#include "mx_gemm.h"
+#include "tc_util.cuh"
+
+namespace tmt {
+namespace {
+
+using namespace tc;
+using namespace mx;
+
+constexpr int kBP = 128;                 // rows of a tile on the P side
+constexpr int kKB = 256;                 // elements of k per pipeline stage: one 128-byte swizzle row, two scale tiles
+constexpr int kMaxExperts = 256;
+constexpr int kThreads = 224;
+
+template <int BN> struct Shape {
+    static constexpr int kQBands = (BN + 127) / 128;                     // 128-row bands of scale tiles on the Q side
+    static constexpr int kCodesP = kBP * 128, kCodesQ = BN * 128;
+    static constexpr int kSfP = 2 * kScaleTile, kSfQ = 2 * kScaleTile * kQBands;
+    static constexpr int kStageBytes = kCodesP + kCodesQ + kSfP + kSfQ;
+    static constexpr int kStages = (200 * 1024) / kStageBytes;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr uint32_t kSfCol = 2 * BN;                           // scale columns follow the two accumulators
+    static constexpr uint32_t kCols = 2 * BN + 8 + 8 * kQBands <= 128 ? 128 : 2 * BN + 8 + 8 * kQBands <= 256 ? 256 : 512;
+    static_assert(2 * BN + 8 + 8 * kQBands <= 512, "tensor memory has 512 columns");
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// 512-byte scale tile in shared memory: 32 rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t dp, uint64_t dq, uint32_t idesc, uint32_t sfp, uint32_t sfq, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(sfp), "r"(sfq), "r"(accumulate) : "memory");
+}
+
+struct Groups {                          // in shared memory: the experts' groups and their tiles on the activation side
+    int first[kMaxExperts + 1];          // first activation tile of each group
+    int poff[kMaxExperts], count[kMaxExperts];
+};
+struct Tile {
+    int expert, row0, rows, w0;          // activation rows [row0, row0 + rows), weight rows from w0
+};
+
+template <int TA>                        // activation rows of a tile
+__device__ __forceinline__ void load_groups(const MxGemm& p, Groups& g) {
+    if (p.experts == 0) {
+        if (threadIdx.x == 0) { g.first[0] = 0; g.first[1] = (p.rows + TA - 1) / TA; g.poff[0] = 0; g.count[0] = p.rows; }
+        return;
+    }
+    for (int e = threadIdx.x; e < p.experts; e += kThreads) {
+        const int r0 = p.poff[e];
+        int c = p.counts[e];
+        if (r0 < 0 || (r0 & 127) || c < 0 || (long)r0 + c > p.row_limit) { report(p.status, kErrSlotRange); c = 0; }
+        g.poff[e] = r0; g.count[e] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {              // prefix sum over the experts, 32 at a time
+        int base = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + threadIdx.x;
+            const int t = e < p.experts ? (g.count[e] + TA - 1) / TA : 0;
+            int incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if ((int)threadIdx.x >= o) incl += v;
+            }
+            if (e < p.experts) g.first[e] = base + incl - t;
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (threadIdx.x == 0) g.first[p.experts] = base;
+    }
+}
+template <int TA, int TW>
+__device__ __forceinline__ bool get_tile(const MxGemm& p, const Groups& g, int t, int w_tiles, Tile& ti) {
+    const int ng = p.experts == 0 ? 1 : p.experts;
+    const int at = t / w_tiles;
+    if (at >= g.first[ng]) return false;
+    int lo = 0, hi = ng;                 // last expert whose first tile is <= at and that has tiles
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (g.first[mid] <= at) lo = mid; else hi = mid; }
+    const int off = (at - g.first[lo]) * TA;
+    ti.expert = lo;
+    ti.row0 = g.poff[lo] + off;
+    ti.rows = min(TA, g.count[lo] - off);
+    ti.w0 = (t - at * w_tiles) * TW;
+    return true;
+}
+
+// ---- epilogues of one warp: its 32 TMEM lanes, all columns of the tile ----
+
+// 32 neighbouring outputs of one activation row. `word` collects the scale bytes of 4 blocks.
+template <int EPI>
+__device__ __forceinline__ void drain_chunk(const MxGemm& p, long row, int col0, float gate, float (&v)[32], uint32_t& word) {
+    if constexpr (EPI == kMxUp) {            // one block (n is a multiple of 64 here)
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) { v[i] *= sigmoid_fast(v[i]); m = max(m, __float_as_uint(v[i]) & 0x7fffffffu); }
+        const uint32_t sb = scale_byte<kE2M1>(m);
+        const float inv = inv_scale(sb);
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = v[8 * j + i] * inv;
+            q[j] = sb == 255u ? 0u : pack_e2m1x8(f);
+        }
+        stg16(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col0 / 2, make_uint4(q[0], q[1], q[2], q[3]));
+        const int k4 = (col0 >> 5) & 3;
+        word |= sb << (8 * k4);
+        if (k4 == 3 || col0 + 32 >= p.n) {
+            *reinterpret_cast<uint32_t*>(p.out_scales + scale_word(row, col0 >> 7, scale_tiles_k(p.n))) = word;
+            word = 0;
+        }
+    } else if constexpr (EPI == kMxF32) {
+        float* dst = static_cast<float*>(p.out) + row * p.n + col0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (col0 + q * 4 < p.n) *reinterpret_cast<float4*>(dst + q * 4) = make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+    } else {
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.n + col0;
+        if constexpr (EPI == kMxDown) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= gate;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (col0 + q * 8 < p.n)
+                stg16(dst + q * 8, make_uint4(pack_bf2(v[q * 8], v[q * 8 + 1]), pack_bf2(v[q * 8 + 2], v[q * 8 + 3]),
+                                              pack_bf2(v[q * 8 + 4], v[q * 8 + 5]), pack_bf2(v[q * 8 + 6], v[q * 8 + 7])));
+    }
+}
+
+// Many rows: lane = activation row, columns = outputs.
+template <int EPI, int BN>
+__device__ __forceinline__ void drain_rows(const MxGemm& p, const Tile& ti, uint32_t tm, int r) {
+    const long row = (long)ti.row0 + r;
+    const bool row_ok = r < ti.rows;
+    float gate = 0.0f;
+    if constexpr (EPI == kMxDown) gate = row_ok ? p.row_scale[row] : 0.0f;
+    uint32_t word = 0;
+#pragma unroll 1
+    for (int cc = 0; cc < BN / 32; ++cc) {
+        const int col0 = ti.w0 + cc * 32;
+        if (col0 >= p.n) break;
+        float v[32];
+        __syncwarp();
+        tmem_ld32(tm + (uint32_t)(cc * 32), v);
+        if (row_ok) drain_chunk<EPI>(p, row, col0, gate, v, word);
+    }
+}
+
+// Few rows: lane = output (a weight row), columns = activation rows.
+template <int EPI, int BN>
+__device__ __forceinline__ void drain_cols(const MxGemm& p, const Tile& ti, uint32_t tm, int o, int lane) {
+    const int col = ti.w0 + o;
+    const bool col_ok = col < p.n;
+    const unsigned full = 0xffffffffu;
+#pragma unroll 1
+    for (int cc = 0; cc < BN / 32; ++cc) {
+        if (cc * 32 >= ti.rows) break;
+        float v[32];
+        tmem_ld32(tm + (uint32_t)(cc * 32), v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (cc * 32 + i >= ti.rows) break;
+            const long row = (long)ti.row0 + cc * 32 + i;
+            if constexpr (EPI == kMxUp) {        // the warp's 32 outputs are one block (col - lane is a multiple of 32)
+                const float s = v[i] * sigmoid_fast(v[i]);
+                const uint32_t m = __reduce_max_sync(full, __float_as_uint(s) & 0x7fffffffu);
+                const uint32_t sb = scale_byte<kE2M1>(m);
+                float f[8] = {s * inv_scale(sb), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t q = sb == 255u ? 0u : (pack_e2m1x8(f) & 15u) << (4 * (lane & 7));
+                q |= __shfl_xor_sync(full, q, 1);
+                q |= __shfl_xor_sync(full, q, 2);
+                q |= __shfl_xor_sync(full, q, 4);
+                if (col_ok) {
+                    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col / 2) = q;
+                    if (lane == 0) p.out_scales[scale_word(row, col >> 7, scale_tiles_k(p.n)) + ((col >> 5) & 3)] = (uint8_t)sb;
+                }
+            } else if constexpr (EPI == kMxF32) {
+                if (col_ok) static_cast<float*>(p.out)[row * p.n + col] = v[i];
+            } else {
+                const float x = EPI == kMxDown ? v[i] * __ldg(p.row_scale + row) : v[i];
+                if (col_ok) static_cast<uint16_t*>(p.out)[row * p.n + col] = f2bf(x);
+            }
+        }
+    }
+}
+
+template <int BN, bool FEW, int EPI>
+__global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_constant__ MxGemm p) {
+    using S = Shape<BN>;
+    constexpr int TA = FEW ? BN : kBP, TW = FEW ? kBP : BN;       // activation / weight rows of a tile
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full_bar[S::kStages], empty_bar[S::kStages], tfull_bar[2], tempty_bar[2];
+    __shared__ Groups groups;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t codes_p = base, codes_q = base + S::kStages * S::kCodesP, sf_p = codes_q + S::kStages * S::kCodesQ, sf_q = sf_p + S::kStages * S::kSfP;
+    volatile int* abort_flag = &abort_s;
+
+    pdl_begin();
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&empty_bar[s]), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(S::kCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    load_groups<TA>(p, groups);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_s;
+    const int w_tiles = (p.n + TW - 1) / TW;
+    const int nkb = (p.k + kKB - 1) / kKB;
+    const int tiles_k = scale_tiles_k(p.k);
+
+    if (warp == 0 || warp == 6) {
+        // ---------------- producers: codes box and scale tiles of one operand per stage ----------------
+        if (lane == 0) {
+            const bool is_p = warp == 0;
+            const bool is_act = is_p != FEW;
+            int s = 0; uint32_t ph = 0;
+            uint32_t issued = 0, last_parity = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok; t += gridDim.x) {
+                Tile ti;
+                if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+                const CUtensorMap* map;
+                const uint8_t* sc;
+                int row;
+                long band;                                     // first 128-row band of scale tiles
+                int bands = 1;
+                if (is_act) {
+                    map = &p.act; sc = p.act_scales; row = ti.row0;
+                } else {
+                    map = p.w_maps ? p.w_maps + ti.expert : &p.w;
+                    sc = p.w_scales_tab ? p.w_scales_tab[ti.expert] : p.w_scales;
+                    row = ti.w0;
+                    if (p.w_maps) tensormap_acquire(map);
+                }
+                band = row >> 7;
+                if (!is_p) bands = min(S::kQBands, is_act ? 1 : (p.n - row + 127) / 128);
+                for (int kb = 0; kb < nkb; ++kb) {
+                    ok = mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, p.status);
+                    if (!ok) break;
+                    const uint32_t fb = smem_u32(&full_bar[s]);
+                    const uint32_t sf_bytes = (uint32_t)min(2, tiles_k - 2 * kb) * kScaleTile;
+                    if (FEW && !is_p) {                        // only the 32-row boxes that hold rows of this tile
+                        const int boxes = (ti.rows + kMxFewRows - 1) / kMxFewRows;
+                        mbar_expect_tx(fb, boxes * (kMxFewRows * 128) + sf_bytes);
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_2d(codes_q + s * S::kCodesQ + b * (kMxFewRows * 128), map, fb, kb * 128, row + b * kMxFewRows);
+                    } else {
+                        mbar_expect_tx(fb, (is_p ? S::kCodesP : S::kCodesQ) + bands * sf_bytes);
+                        tma_load_2d(is_p ? codes_p + s * S::kCodesP : codes_q + s * S::kCodesQ, map, fb, kb * 128, row);
+                    }
+                    const uint32_t sf = is_p ? sf_p + s * S::kSfP : sf_q + s * S::kSfQ;
+                    for (int b = 0; b < bands; ++b)
+                        bulk_load(sf + b * 2 * kScaleTile, sc + ((size_t)(band + b) * tiles_k + 2 * kb) * kScaleTile, sf_bytes, fb);
+                    issued |= 1u << s;
+                    last_parity = (last_parity & ~(1u << s)) | (ph << s);
+                    if (++s == S::kStages) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok)       // aborting: wait (bounded) until the copies already issued have landed
+                for (int q = 0; q < S::kStages; ++q) {
+                    if (!(issued >> q & 1)) continue;
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(smem_u32(&full_bar[q]), (last_parity >> q) & 1) && clock64() - t0 < kWaitCycles) {}
+                }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: the whole warp runs the loop, one elected lane issues ----------------
+        // e2m1 operands, e8m0 scales, both K-major; the scale ids (0 or 2) pick the blocks 0-1 or 2-3 of a tile
+        const uint32_t idesc_mn = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kBP >> 4) << 24);
+        const uint32_t sfp_t = tmem_base + S::kSfCol, sfq_t = sfp_t + 8;
+        int s = 0; uint32_t ph = 0;
+        int acc = 0; uint32_t acc_ph = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok; t += gridDim.x) {
+            Tile ti;
+            if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tempty_bar[acc]), acc_ph ^ 1, abort_flag, p.status));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + acc * BN;
+            // few rows: as many columns as the tile has rows. A tile starts on a 128-row band of scales, so the scale columns of
+            // an MMA always start on a whole tile's first column (a start inside a tile is not a form this kernel relies on).
+            const uint32_t cols_q = FEW ? (uint32_t)((ti.rows + kMxFewRows - 1) / kMxFewRows * kMxFewRows) : (uint32_t)BN;
+            const uint32_t idesc0 = idesc_mn | ((cols_q >> 3) << 17);
+            for (int kb = 0; kb < nkb; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, p.status));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t dp = make_desc(codes_p + s * S::kCodesP, false, 0), dq = make_desc(codes_q + s * S::kCodesQ, false, 0);
+                    const int steps = min(4, (p.k - kb * kKB) / 64);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        if (2 * a < steps) {
+                            scale_copy(sfp_t + a * 4, scale_desc(sf_p + s * S::kSfP + a * kScaleTile));
+#pragma unroll
+                            for (int b = 0; b < S::kQBands; ++b)
+                                scale_copy(sfq_t + a * 4 * S::kQBands + b * 4, scale_desc(sf_q + s * S::kSfQ + b * 2 * kScaleTile + a * kScaleTile));
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < steps) {
+                            const uint32_t id = (j & 1) * 2;
+                            mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | (id << 4) | (id << 29), sfp_t + (j >> 1) * 4,
+                                     sfq_t + (j >> 1) * 4 * S::kQBands, (kb | j) != 0);
+                        }
+                    tc_commit(smem_u32(&empty_bar[s]));
+                }
+                __syncwarp();
+                if (++s == S::kStages) { s = 0; ph ^= 1; }
+            }
+            if (!ok) break;
+            if (elect_one()) tc_commit(smem_u32(&tfull_bar[acc]));
+            __syncwarp();
+            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- epilogue ----------------
+        const int quarter = warp & 3;
+        int acc = 0; uint32_t acc_ph = 0;
+        for (int t = blockIdx.x;; t += gridDim.x) {
+            Tile ti;
+            if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[acc]), acc_ph, abort_flag, p.status))) break;
+            tc_fence_after();
+            const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
+            if constexpr (FEW) drain_cols<EPI, BN>(p, ti, tm, quarter * 32 + lane, lane);
+            else drain_rows<EPI, BN>(p, ti, tm, quarter * 32 + lane);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kCols) : "memory");
+    }
+}
+
+template <int BN, bool FEW, int EPI>
+cudaError_t launch_t(const MxGemm& p, int grid, cudaStream_t stream) {
+    constexpr int smem = Shape<BN>::kSmem;
+    const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<BN, FEW, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(mx_gemm_kernel<BN, FEW, EPI>, dim3(grid), dim3(kThreads), smem, stream, p);
+}
+template <int BN, bool FEW>
+cudaError_t launch_epi(const MxGemm& p, int grid, cudaStream_t stream) {
+    switch (p.epi) {
+        case kMxBf16: return launch_t<BN, FEW, kMxBf16>(p, grid, stream);
+        case kMxF32: return launch_t<BN, FEW, kMxF32>(p, grid, stream);
+        case kMxUp: return launch_t<BN, FEW, kMxUp>(p, grid, stream);
+        case kMxDown: return launch_t<BN, FEW, kMxDown>(p, grid, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    if (!fn) throw std::runtime_error("cuTensorMapEncodeTiled is not available from this driver");
+    return fn;
+}
+
+}  // namespace
+
+bool mx_few_rows(long rows_per_group) { return rows_per_group <= 32; }
+
+void mx_make_map(CUtensorMap* m, const void* codes, uint64_t rows, int cols, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols / 2, rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)cols / 2};
+    const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed for a 4-bit matrix (" + std::to_string((int)r) + ")");
+}
+
+cudaError_t launch_mx_gemm(const MxGemm& p, int num_sms, cudaStream_t stream) {
+    return p.few_rows ? launch_epi<128, true>(p, num_sms, stream) : launch_epi<128, false>(p, num_sms, stream);
+}
+
+}  // namespace tmt

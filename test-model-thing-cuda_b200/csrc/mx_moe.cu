@@ -1,0 +1,254 @@
+// Entry points of the 4-bit products (include/tmt_mx.h): the dense layer, and the block's forward pass with both expert
+// products on 4-bit blocks. Router, offset tables and combine are those of tmt_moe_forward; between them run the
+// quantising dispatch below and two grouped products (mx_gemm.cu): up writes q4(silu(.)) straight from its accumulators,
+// down applies the gate weight.
+#include <algorithm>
+#include <cstring>
+
+#include "../../include/tmt_mx.h"
+#include "launch_pdl.cuh"
+#include "moe_internal.h"
+#include "mx.cuh"
+#include "mx_cast.h"
+#include "mx_gemm.h"
+#include "mx_host.h"
+
+namespace tmt {
+namespace {
+
+using namespace mx;
+
+constexpr int kDispatchWarps = 8;
+constexpr int kMaxTopk = 8;
+
+// One warp per token: the row is read and quantised once, its codes and scale words are written to the token's K rows of
+// the experts' groups (topk * 0.53 bytes per element instead of the bf16 dispatch's topk * 2). Rows between a group's end and
+// its padding keep what they held: the products neither use nor write them.
+__global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const RouteDims d, const RouteBufs b, const uint16_t* __restrict__ X,
+                                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    extern __shared__ int table[];       // [E] first row of this router block's assignments to each expert
+    pdl_begin();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned full = 0xffffffffu;
+    // kTokBlock is a multiple of the 8 tokens of this block, so one router block covers them all
+    const long t0 = (long)blockIdx.x * kDispatchWarps;
+    const int rb = (int)(t0 / kTokBlock);
+    for (int e = threadIdx.x; e < d.E; e += blockDim.x) table[e] = b.poff[e] + b.block_base[(long)rb * d.E + e];
+    __syncthreads();
+    const long t = t0 + warp;
+    if (t >= d.T) return;
+    int slot = -1;
+    if (lane < d.K) {
+        const int e = b.idx[t * d.K + lane];
+        if (e < 0 || e >= d.E) report(b.status, kErrSlotRange);
+        else {
+            slot = table[e] + b.rank[t * d.K + lane];
+            if (slot < 0 || slot >= d.cap) { report(b.status, kErrSlotRange); slot = -1; }
+            else {
+                b.slot_of[t * d.K + lane] = slot;
+                b.slotw[slot] = b.w[t * d.K + lane];
+                b.tok_of_slot[slot] = (int)t;
+            }
+        }
+    }
+    int slots[kMaxTopk];
+#pragma unroll
+    for (int j = 0; j < kMaxTopk; ++j) slots[j] = __shfl_sync(full, slot, j);
+    const uint16_t* src = X + t * d.D;
+    const int tiles_k = scale_tiles_k(d.D);
+    for (int c0 = 0; c0 < d.D; c0 += 256) {
+        const int col = c0 + lane * 8;
+        const bool ok = col < d.D;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (ok) x = ldg16(src + col);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        float f[8];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); m = __vmaxu2(m, w[i] & 0x7fff7fffu); }
+        m = max(m >> 16, m & 0xffffu) << 16;
+        m = max(m, __shfl_xor_sync(full, m, 1));
+        m = max(m, __shfl_xor_sync(full, m, 2));
+        const uint32_t sb = scale_byte<kE2M1>(m);
+        const float inv = inv_scale(sb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= inv;
+        const uint32_t q = sb == 255u ? 0u : pack_e2m1x8(f);
+        uint32_t word = ok ? sb << (8 * ((lane >> 2) & 3)) : 0u;
+        word |= __shfl_xor_sync(full, word, 4);
+        word |= __shfl_xor_sync(full, word, 8);
+        if (ok) {
+#pragma unroll
+            for (int j = 0; j < kMaxTopk; ++j)
+                if (j < d.K && slots[j] >= 0) {
+                    *reinterpret_cast<uint32_t*>(codes + ((long)slots[j] * d.D + col) / 2) = q;
+                    if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(slots[j], col >> 7, tiles_k)) = word;
+                }
+        }
+    }
+}
+
+template <class T>
+T* alloc(tmt_moe* h, size_t n) {
+    void* p = nullptr;
+    cuda_ok(cudaMalloc(&p, n * sizeof(T)), "cudaMalloc");
+    h->allocs.push_back(p);
+    h->bytes += n * sizeof(T);
+    return static_cast<T*>(p);
+}
+
+void make_buffers(tmt_moe* h) {
+    MxState& m = h->mx;
+    if (m.tables) return;
+    const int D = h->d.dim, H = h->d.hidden, E = h->d.experts;
+    const long cap = h->dims.cap;
+    m.x_codes = alloc<uint8_t>(h, (size_t)cap * D / 2);
+    m.x_scales = alloc<uint8_t>(h, scale_bytes(cap, D));
+    m.h_codes = alloc<uint8_t>(h, (size_t)cap * H / 2);
+    m.h_scales = alloc<uint8_t>(h, scale_bytes(cap, H));
+    for (int few = 0; few < 2; ++few) {
+        mx_make_map(&m.x_map[few], m.x_codes, cap, D, few ? kMxFewRows : kMxMapRows);
+        mx_make_map(&m.h_map[few], m.h_codes, cap, H, few ? kMxFewRows : kMxMapRows);
+    }
+    // the padding rows' scale bytes are read with the others (their products are never used): give them a value
+    cuda_ok(cudaMemsetAsync(m.x_scales, 0, scale_bytes(cap, D), h->stream), "cudaMemsetAsync");
+    cuda_ok(cudaMemsetAsync(m.h_scales, 0, scale_bytes(cap, H), h->stream), "cudaMemsetAsync");
+    m.tables = alloc<CUtensorMap>(h, 2 * (size_t)E);
+    m.scale_tab = alloc<const uint8_t*>(h, 2 * (size_t)E);
+}
+
+// Per-expert maps and scale pointers, uploaded when the caller's pointers changed.
+void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown) {
+    const int E = h->d.experts;
+    MxState& m = h->mx;
+    std::vector<const void*> key(4 * (size_t)E);
+    for (int e = 0; e < E; ++e) { key[e] = Wup[e].scales; key[E + e] = Wdown[e].scales; key[2 * E + e] = Wup[e].codes; key[3 * E + e] = Wdown[e].codes; }
+    if (key == m.key) return;
+    m.key.clear();                       // stays empty if anything below throws
+    for (const void* p : key) check_tensors({p});
+    std::vector<CUtensorMap> maps(2 * (size_t)E);
+    for (int e = 0; e < E; ++e) {
+        mx_make_map(&maps[e], Wup[e].codes, Wup[e].rows, Wup[e].cols, kMxMapRows);
+        mx_make_map(&maps[E + e], Wdown[e].codes, Wdown[e].rows, Wdown[e].cols, kMxMapRows);
+    }
+    cuda_ok(cudaMemcpyAsync(m.tables, maps.data(), maps.size() * sizeof(CUtensorMap), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
+    cuda_ok(cudaMemcpyAsync(m.scale_tab, key.data(), 2 * (size_t)E * sizeof(void*), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
+    cuda_ok(cudaStreamSynchronize(h->stream), "cudaStreamSynchronize");      // the host vectors are about to go
+    m.key = key;
+}
+
+void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown, void* Y,
+                float beta, int tokens) {
+    const int D = h->d.dim, H = h->d.hidden, E = h->d.experts, K = h->d.topk;
+    if (H == 0 || h->d.training || h->d.ep_world > 1) throw std::runtime_error("MXFP4 forward needs hidden > 0, training = 0 and a single rank");
+    if (!X || !Wr || !Wup || !Wdown || !Y) throw std::runtime_error("null argument");
+    if (tokens < 1 || tokens > h->d.tokens) throw std::runtime_error("tokens outside [1, desc.tokens]");
+    for (int e = 0; e < E; ++e)
+        if (Wup[e].rows != H || Wup[e].cols != D || Wdown[e].rows != D || Wdown[e].cols != H)
+            throw std::runtime_error("MXFP4 weight shape does not match the handle");
+    cuda_ok(cudaSetDevice(h->d.device), "cudaSetDevice");
+    make_buffers(h);
+    refresh_tables(h, Wup, Wdown);
+    MxState& m = h->mx;
+    h->dims.T = tokens;
+    h->last_tokens = tokens;
+    route_only(h, static_cast<const uint16_t*>(X), Wr);
+    prof_mark(h, kPhDispatch);
+    cuda_ok(launch_pdl(mx_dispatch_kernel, dim3((tokens + kDispatchWarps - 1) / kDispatchWarps), dim3(kDispatchWarps * 32), E * sizeof(int),
+                       h->stream, h->dims, h->rb, static_cast<const uint16_t*>(X), m.x_codes, m.x_scales), "mx dispatch launch");
+    MxGemm p;
+    memset(&p, 0, sizeof p);
+    p.experts = E; p.poff = h->rb.poff; p.counts = h->rb.counts; p.row_limit = h->dims.cap;
+    p.status = h->rb.status;
+    p.few_rows = mx_few_rows(((long)tokens * K + E - 1) / E);
+    p.act = m.x_map[p.few_rows]; p.act_scales = m.x_scales;
+    p.w_maps = m.tables; p.w_scales_tab = m.scale_tab;
+    p.n = H; p.k = D; p.epi = kMxUp; p.out = m.h_codes; p.out_scales = m.h_scales;
+    prof_mark(h, kPhGemmUp);
+    cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
+    p.act = m.h_map[p.few_rows]; p.act_scales = m.h_scales;
+    p.w_maps = m.tables + E; p.w_scales_tab = m.scale_tab + E;
+    p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.row_scale = h->rb.slotw;
+    prof_mark(h, kPhGemmDown);
+    cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx down launch");
+    prof_mark(h, kPhCombine);
+    cuda_ok(launch_combine(h->dims, h->rb, h->Yg, static_cast<uint16_t*>(Y), beta, 0, h->stream), "combine launch");
+    prof_mark(h, -1);
+    h->launches += 4;
+    h->have_forward = true;
+}
+
+void check_weight(const tmt_mxfp4_weight* W) {
+    if (!W) throw std::runtime_error("null argument");
+    if (W->rows < 8 || W->rows % 8 || W->cols < 64 || W->cols % 64)
+        throw std::runtime_error("MXFP4 weight: rows must be a positive multiple of 8, cols of 64");
+}
+
+void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
+    MxGemm p;
+    memset(&p, 0, sizeof p);
+    p.few_rows = mx_few_rows(rows);
+    mx_make_map(&p.act, codes, rows, W.cols, p.few_rows ? kMxFewRows : kMxMapRows);
+    mx_make_map(&p.w, W.codes, W.rows, W.cols, kMxMapRows);
+    p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
+    p.rows = rows; p.n = W.rows; p.k = W.cols;
+    p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
+    cuda_ok(launch_mx_gemm(p, sm_count(), s), "matmul_mxfp4 launch");
+}
+
+void check_dtype(int dtype) {
+    if (dtype != TMT_MOE_BF16 && dtype != TMT_MOE_F32) throw std::runtime_error("dtype must be TMT_MOE_BF16 or TMT_MOE_F32");
+}
+
+// codes first, then the scale tiles on a 16-byte boundary (cols / 2 is a multiple of 32)
+size_t codes_bytes(long long rows, int cols) { return (size_t)rows * cols / 2; }
+
+}  // namespace
+}  // namespace tmt
+
+using namespace tmt;
+
+extern "C" {
+
+int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, const tmt_mxfp4_weight* W, void* Y, int dtype,
+                         int* status, void* stream) {
+    MX_GUARD({
+        check_weight(W);
+        check_dtype(dtype);
+        if (rows < 0) throw std::runtime_error("rows must not be negative");
+        if (rows == 0) return 0;
+        check_tensors({A_codes, A_scales, W->codes, W->scales, Y});
+        matmul(A_codes, A_scales, rows, *W, Y, dtype, status, static_cast<cudaStream_t>(stream));
+    })
+}
+
+size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols) {
+    return rows < 0 || cols < 64 || cols % 64 ? 0 : codes_bytes(rows, cols) + mx::scale_bytes((long)rows, cols);
+}
+
+int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
+                         size_t work_bytes, int* status, void* stream) {
+    MX_GUARD({
+        check_weight(W);
+        check_dtype(x_dtype);
+        check_dtype(y_dtype);
+        if (rows < 0) throw std::runtime_error("rows must not be negative");
+        if (rows == 0) return 0;
+        if (work_bytes < tmt_moe_linear_mxfp4_work_bytes(rows, W->cols)) throw std::runtime_error("work buffer too small (tmt_moe_linear_mxfp4_work_bytes)");
+        check_tensors({X, W->codes, W->scales, Y, work});
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        uint8_t* codes = static_cast<uint8_t*>(work);
+        uint8_t* scales = codes + codes_bytes(rows, W->cols);
+        cuda_ok(launch_mx4_quantize(X, x_dtype == TMT_MOE_F32, rows, W->cols, codes, scales, s, true), "quantize_mxfp4 launch");
+        matmul(codes, scales, rows, *W, Y, y_dtype, status, s);
+    })
+}
+
+int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown,
+                          void* Y, float beta, int tokens) {
+    if (!h) { set_error("null handle"); return -1; }
+    MX_GUARD(forward_mx(h, X, Wrouter, Wup, Wdown, Y, beta, tokens))
+}
+
+}  // extern "C"

@@ -9,10 +9,8 @@
 
 #include "../../include/tmt_norm.h"
 #include "common.cuh"
-
-namespace tmt {
-void set_error(const char* fmt, ...);
-}
+#include "mx.cuh"
+#include "mx_host.h"
 
 namespace {
 
@@ -40,10 +38,13 @@ __device__ __forceinline__ float butterfly(float v) {
 
 // One warp per row (rows taken grid-stride); the row stays in registers between the statistics and the output (one
 // read of X) and the next row is fetched before the current one is reduced.
-template <int NV>
+// FMT: mx::kE4M3 / mx::kE5M2 leaves an 8-bit checkpoint of the row as well (a block of 32 is the vectors of 4 neighbouring
+// lanes): one byte more per element written, and no second read of X. 0: none.
+template <int NV, int FMT>
 __global__ void __launch_bounds__(kFwdWarps * 32) ln_fwd_kernel(const uint16_t* __restrict__ X, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, uint16_t* __restrict__ Y,
-                                                                float* __restrict__ mean, float* __restrict__ rstd, int rows, int D) {
+                                                                float* __restrict__ mean, float* __restrict__ rstd, int rows, int D,
+                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     const int lane = threadIdx.x & 31;
     const int nvec = D >> 3;
     const long stride = (long)gridDim.x * kFwdWarps;
@@ -97,6 +98,32 @@ __global__ void __launch_bounds__(kFwdWarps * 32) ln_fwd_kernel(const uint16_t* 
 #pragma unroll
                 for (int q = 0; q < 8; ++q) o[q] = __fmaf_rn(__fmul_rn(__fsub_rn(f[q], m), rs), gg[q], bb[q]);
                 stg16(y + v * 8, make_uint4(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]), pack_bf2(o[4], o[5]), pack_bf2(o[6], o[7])));
+            }
+        }
+        if constexpr (FMT != 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int v = lane + i * 32;
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                uint32_t m = 0;                       // magnitudes of bf16 order like their bits
+                if (v < nvec) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) m = __vmaxu2(m, w[q] & 0x7fff7fffu);
+                }
+                m = max(m >> 16, m & 0xffffu) << 16;
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                if (v < nvec) {                       // dim is a multiple of 32: the four lanes of a block agree
+                    const uint32_t sb = mx::scale_byte<FMT>(m);
+                    const float inv = mx::inv_scale(sb);
+                    float f[8];
+                    unpack8(raw[i], f);
+                    uint32_t lo = mx::pack_f8x4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+                    uint32_t hi = mx::pack_f8x4<FMT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                    if (sb == 255u) { lo = 0; hi = 0; }
+                    *reinterpret_cast<uint2*>(codes + r * D + v * 8) = make_uint2(lo, hi);
+                    if ((lane & 3) == 0) scales[r * (D >> 5) + (v >> 2)] = (uint8_t)sb;
+                }
             }
         }
         if constexpr (kPrefetch) {
@@ -302,6 +329,27 @@ void check_shape(int rows, int dim, int max_dim) {
         throw std::runtime_error("need rows >= 1 and dim a multiple of 8, at most " + std::to_string(max_dim));
 }
 
+template <int FMT>
+void launch_ln_fwd(const void* X, const float* gamma, const float* beta, void* Y, float* mean, float* rstd, int rows, int dim,
+                   uint8_t* codes, uint8_t* scales, void* stream) {
+    const int nv = (dim / 8 + 31) / 32;
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int want = (rows + kFwdWarps - 1) / kFwdWarps;
+    const dim3 grid(std::max(1, std::min(want, std::max(sms, 1) * 6))), block(kFwdWarps * 32);      // a multiple of the SM count
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const uint16_t* x = static_cast<const uint16_t*>(X);
+    uint16_t* y = static_cast<uint16_t*>(Y);
+    if (nv <= 2) ln_fwd_kernel<2, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 4) ln_fwd_kernel<4, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 8) ln_fwd_kernel<8, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 16) ln_fwd_kernel<16, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else ln_fwd_kernel<kFwdMaxVec, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) throw std::runtime_error(std::string("LayerNorm forward launch failed: ") + cudaGetErrorString(e));
+}
+
 }  // namespace
 
 extern "C" {
@@ -311,24 +359,25 @@ int tmt_ln_forward(const void* X, const float* gamma, const float* beta, void* Y
     try {
         if (!X || !gamma || !beta || !Y || !mean || !rstd) throw std::runtime_error("null argument");
         check_shape(rows, dim, 32 * kFwdMaxVec * 8);
-        const int nv = (dim / 8 + 31) / 32;
-        int dev = 0, sms = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        const int want = (rows + kFwdWarps - 1) / kFwdWarps;
-        const dim3 grid(std::max(1, std::min(want, std::max(sms, 1) * 6))), block(kFwdWarps * 32);      // a multiple of the SM count
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const uint16_t* x = static_cast<const uint16_t*>(X);
-        uint16_t* y = static_cast<uint16_t*>(Y);
-        if (nv <= 2) ln_fwd_kernel<2><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim);
-        else if (nv <= 4) ln_fwd_kernel<4><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim);
-        else if (nv <= 8) ln_fwd_kernel<8><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim);
-        else if (nv <= 16) ln_fwd_kernel<16><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim);
-        else ln_fwd_kernel<kFwdMaxVec><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim);
-        const cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) throw std::runtime_error(std::string("LayerNorm forward launch failed: ") + cudaGetErrorString(e));
+        launch_ln_fwd<0>(X, gamma, beta, Y, mean, rstd, rows, dim, nullptr, nullptr, stream);
         return 0;
     } catch (const std::exception& e) { set_error("%s", e.what()); return -1; }
+}
+
+int tmt_ln_forward_act8(const void* X, const float* gamma, const float* beta, void* Y, float* mean, float* rstd, void* codes,
+                        void* scales, int format, int rows, int dim, void* stream) {
+    MX_GUARD({
+        if (rows == 0) return 0;
+        check_shape(rows, dim, 32 * kFwdMaxVec * 8);
+        if (dim % 32) throw std::runtime_error("an 8-bit checkpoint needs dim to be a multiple of 32");
+        check_tensors({X, gamma, beta, Y, codes, scales});
+        check_tensors({mean, rstd}, 4);
+        uint8_t* c = static_cast<uint8_t*>(codes);
+        uint8_t* sc = static_cast<uint8_t*>(scales);
+        if (format == mx::kE4M3) launch_ln_fwd<mx::kE4M3>(X, gamma, beta, Y, mean, rstd, rows, dim, c, sc, stream);
+        else if (format == mx::kE5M2) launch_ln_fwd<mx::kE5M2>(X, gamma, beta, Y, mean, rstd, rows, dim, c, sc, stream);
+        else throw std::runtime_error("format must be TMT_ACT8_E4M3 or TMT_ACT8_E5M2");
+    })
 }
 
 size_t tmt_ln_backward_scratch_bytes(int rows, int dim) {

@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libtmt_moe_b200.so")
 BF16, F32 = 0, 1
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05_2CTA, GEMM_TCGEN05 = 0, 1, 2, 3
 EP_PEER, EP_NCCL, EP_DMA = 0, 1, 2
+ACT8_OFF, ACT8_E4M3, ACT8_E5M2 = 0, 1, 2
 
 EXPORTS = (
     "tmt_moe_create", "tmt_moe_destroy", "tmt_moe_last_error", "tmt_moe_set_router_bias",
@@ -35,6 +36,9 @@ EXPORTS = (
     "tmt_sampler_create", "tmt_sampler_destroy", "tmt_sampler_set_weights", "tmt_sampler_x", "tmt_sampler_y",
     "tmt_sampler_stream", "tmt_sampler_step", "tmt_sampler_upload", "tmt_sampler_download", "tmt_sampler_sync",
     "tmt_sampler_sample", "tmt_sampler_steps", "tmt_sampler_graphs", "tmt_sampler_set_layernorm",
+    "tmt_moe_mxfp4_scale_bytes", "tmt_moe_quantize_mxfp4", "tmt_moe_dequantize_mxfp4", "tmt_moe_matmul_mxfp4",
+    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_act8_save", "tmt_moe_act8_restore",
+    "tmt_ln_forward_act8", "tmt_ln_backward_act8", "tmt_ln_backward_act8_scratch_bytes",
 )
 
 
@@ -73,6 +77,7 @@ def load():
     lib.tmt_moe_ep_plan.restype = ctypes.c_longlong
     lib.tmt_moe_destroy.restype = None
     lib.tmt_moe_phase_name.restype = ctypes.c_char_p
+    _declare_mx(lib)
     for name in EXPORTS:
         getattr(lib, name)
     _lib = lib
@@ -243,6 +248,22 @@ class MoE:
         keep = (arr(Wup), arr(Wdown))
         _check(self.lib.tmt_moe_forward_nvfp4_ln(self.h, _ptr(X), _ptr(gamma), _ptr(beta_ln), _ptr(Wrouter), keep[0], keep[1],
                                                  _ptr(Y), ctypes.c_float(beta), t), self.lib)
+
+    def forward_mxfp4(self, X, Wrouter, Wup, Wdown, Y, beta=0.0, tokens=None):
+        """forward with both expert products on 4-bit blocks (include/tmt_mx.h). Wup / Wdown: Mxfp4Weights, or lists of
+        (codes, scales, rows, cols), one entry per expert (a Mxfp4Weights kept by the caller saves building it at every call)."""
+        t = self.tokens if tokens is None else tokens
+        up = Wup if isinstance(Wup, Mxfp4Weights) else Mxfp4Weights(Wup)
+        down = Wdown if isinstance(Wdown, Mxfp4Weights) else Mxfp4Weights(Wdown)
+        if up.n != self.experts or down.n != self.experts:
+            raise MoeError("forward_mxfp4 needs one weight per expert (%d), got %d and %d" % (self.experts, up.n, down.n))
+        for name, a in (("X", X), ("Y", Y)):
+            _dense(a, name, ("torch.bfloat16", "torch.int16"))
+            if a.shape[-1] != self.dim or a.numel() < t * self.dim:
+                raise MoeError("%s has too few rows or another width than the handle" % name)
+        _dense(Wrouter, "Wrouter", ("torch.float32",) if self.desc.router_dtype == F32 else ("torch.bfloat16", "torch.int16"))
+        self._mx_keep = (up, down)          # the handle keeps a table of their device addresses
+        _check(self.lib.tmt_moe_forward_mxfp4(self.h, X.data_ptr(), Wrouter.data_ptr(), up.arr, down.arr, Y.data_ptr(), beta, t), self.lib)
 
     def nvfp4_weights_changed(self):
         """Call after re-quantising into the same buffers: derived copies are rebuilt at the next forward_nvfp4."""
@@ -481,3 +502,201 @@ def quantize_nvfp4(W, rows, cols, packed, scales, stream=None):
     _check(lib.tmt_moe_quantize_nvfp4(_ptr(W), rows, cols, _ptr(packed), _ptr(scales), ctypes.byref(ts),
                                       ctypes.c_void_p(stream)), lib)
     return ts.value
+
+
+# ---- microscaled operators (include/tmt_mx.h) ----
+# These calls are made once per layer and step, many of them on a few rows, where the time of the call itself counts: the
+# argument types are declared once, so that plain integers go through ctypes as they are. Tensors are checked here for
+# layout, type and size, on the C side for alignment and device.
+
+class _Mxfp4WeightDesc(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_int), ("cols", ctypes.c_int)]
+
+
+def _declare_mx(lib):
+    vp, i, f, ll, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_size_t
+    wp = ctypes.POINTER(_Mxfp4WeightDesc)
+    for name, res, args in (
+            ("tmt_moe_mxfp4_scale_bytes", sz, [ll, i]), ("tmt_moe_linear_mxfp4_work_bytes", sz, [ll, i]),
+            ("tmt_moe_quantize_mxfp4", i, [vp, i, ll, i, vp, vp, vp]), ("tmt_moe_dequantize_mxfp4", i, [vp, vp, ll, i, vp, i, vp]),
+            ("tmt_moe_matmul_mxfp4", i, [vp, vp, i, wp, vp, i, vp, vp]), ("tmt_moe_linear_mxfp4", i, [vp, i, i, wp, vp, i, vp, sz, vp, vp]),
+            ("tmt_moe_forward_mxfp4", i, [vp, vp, vp, wp, wp, vp, f, i]),
+            ("tmt_moe_act8_save", i, [vp, i, ll, i, i, vp, vp, vp]), ("tmt_moe_act8_restore", i, [vp, vp, ll, i, i, vp, i, vp]),
+            ("tmt_ln_forward_act8", i, [vp] * 8 + [i, i, i, vp]), ("tmt_ln_backward_act8_scratch_bytes", sz, [i, i]),
+            ("tmt_ln_backward_act8", i, [vp, vp, i] + [vp] * 7 + [i, i, vp, vp])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+
+
+_DTYPE = {"torch.bfloat16": BF16, "torch.int16": BF16, "torch.float32": F32}
+_BYTES = ("torch.uint8", "torch.float8_e4m3fn", "torch.float8_e5m2", "torch.float8_e8m0fnu")
+
+
+def _dense(t, name, dtypes):
+    if not t.is_contiguous():
+        raise MoeError("%s must be contiguous" % name)
+    d = str(t.dtype)
+    if d not in dtypes:
+        raise MoeError("%s has type %s, expected %s" % (name, d, " or ".join(dtypes)))
+    return d
+
+
+def _values(t, name):
+    """TMT_MOE_BF16 / TMT_MOE_F32 of a dense matrix of values (int16: raw bf16 patterns, as elsewhere in this package)."""
+    if t.dim() != 2:
+        raise MoeError("%s must have two dimensions" % name)
+    return _DTYPE[_dense(t, name, tuple(_DTYPE))]
+
+
+def _bytes(t, name, need):
+    _dense(t, name, _BYTES)
+    if t.numel() < need:
+        raise MoeError("%s holds %d bytes, %d are needed" % (name, t.numel(), need))
+
+
+class Mxfp4Weights:
+    """Weights of a dense layer (one entry) or of all experts in 4-bit blocks: entries (codes, scales, rows, cols) as quantize_mxfp4
+    leaves them. Keeps the tensors alive."""
+
+    def __init__(self, entries):
+        entries = list(entries)
+        self.n = len(entries)
+        self.arr = (_Mxfp4WeightDesc * self.n)()
+        for i, (c, s, r, k) in enumerate(entries):
+            _bytes(c, "codes", r * k // 2)
+            _bytes(s, "scales", mxfp4_scale_bytes(r, k))
+            self.arr[i] = _Mxfp4WeightDesc(c.data_ptr(), s.data_ptr(), r, k)
+        self._keep = entries
+
+
+def mxfp4_scale_bytes(rows, cols):
+    return int(load().tmt_moe_mxfp4_scale_bytes(rows, cols))
+
+
+def quantize_mxfp4(X, codes, scales, stream=None):
+    """X (rows, cols) bf16 or fp32 -> 4-bit blocks; codes: rows * cols / 2 bytes, scales: mxfp4_scale_bytes(rows, cols) bytes."""
+    lib = load()
+    dt = _values(X, "X")
+    rows, cols = X.shape
+    _bytes(codes, "codes", rows * cols // 2)
+    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
+    _check(lib.tmt_moe_quantize_mxfp4(X.data_ptr(), dt, rows, cols, codes.data_ptr(), scales.data_ptr(), stream), lib)
+
+
+def dequantize_mxfp4(codes, scales, Y, stream=None):
+    """4-bit blocks -> Y (rows, cols) bf16 or fp32."""
+    lib = load()
+    dt = _values(Y, "Y")
+    rows, cols = Y.shape
+    _bytes(codes, "codes", rows * cols // 2)
+    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
+    _check(lib.tmt_moe_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, cols, Y.data_ptr(), dt, stream), lib)
+
+
+def _one_weight(W):
+    W = W if isinstance(W, Mxfp4Weights) else Mxfp4Weights([W])
+    if W.n != 1:
+        raise MoeError("a dense layer has one weight, got %d" % W.n)
+    return W
+
+
+def _out_shape(Y, rows, W):
+    dt = _values(Y, "Y")
+    if tuple(Y.shape) != (rows, W.arr[0].rows):
+        raise MoeError("Y has shape %s, expected %s" % (tuple(Y.shape), (rows, W.arr[0].rows)))
+    return dt
+
+
+def matmul_mxfp4(codes, scales, W, Y, status=None, stream=None):
+    """Y (rows, W rows) = A W^T, both in 4-bit blocks; W: Mxfp4Weights with one entry, or (codes, scales, rows, cols)."""
+    lib = load()
+    W = _one_weight(W)
+    rows, k = Y.shape[0], W.arr[0].cols
+    dt = _out_shape(Y, rows, W)
+    _bytes(codes, "codes", rows * k // 2)
+    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, k))
+    _check(lib.tmt_moe_matmul_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, W.arr, Y.data_ptr(), dt,
+                                    None if status is None else status.data_ptr(), stream), lib)
+
+
+def linear_mxfp4_work_bytes(rows, cols):
+    return int(load().tmt_moe_linear_mxfp4_work_bytes(rows, cols))
+
+
+def linear_mxfp4(X, W, Y, work, status=None, stream=None):
+    """Y = q4(X) W^T: X (rows, cols) bf16 or fp32 is quantised into work (linear_mxfp4_work_bytes(rows, cols) bytes) and multiplied."""
+    lib = load()
+    W = _one_weight(W)
+    xt = _values(X, "X")
+    rows, k = X.shape
+    if k != W.arr[0].cols:
+        raise MoeError("X has %d columns, the weight %d" % (k, W.arr[0].cols))
+    yt = _out_shape(Y, rows, W)
+    _dense(work, "work", _BYTES)
+    _check(lib.tmt_moe_linear_mxfp4(X.data_ptr(), xt, rows, W.arr, Y.data_ptr(), yt, work.data_ptr(), work.numel(),
+                                    None if status is None else status.data_ptr(), stream), lib)
+
+
+def act8_save(X, codes, scales, fmt=ACT8_E4M3, stream=None):
+    """8-bit checkpoint of X (rows, cols) bf16 or fp32; codes: rows * cols bytes, scales: rows * cols / 32 bytes."""
+    lib = load()
+    dt = _values(X, "X")
+    rows, cols = X.shape
+    _bytes(codes, "codes", rows * cols)
+    _bytes(scales, "scales", rows * cols // 32)
+    _check(lib.tmt_moe_act8_save(X.data_ptr(), dt, rows, cols, fmt, codes.data_ptr(), scales.data_ptr(), stream), lib)
+
+
+def act8_restore(codes, scales, Y, fmt=ACT8_E4M3, stream=None):
+    """The values of an 8-bit checkpoint -> Y (rows, cols) bf16 or fp32."""
+    lib = load()
+    dt = _values(Y, "Y")
+    rows, cols = Y.shape
+    _bytes(codes, "codes", rows * cols)
+    _bytes(scales, "scales", rows * cols // 32)
+    _check(lib.tmt_moe_act8_restore(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, Y.data_ptr(), dt, stream), lib)
+
+
+def _ln_checkpoint(codes, scales, rows, dim):
+    _bytes(codes, "codes", rows * dim)
+    _bytes(scales, "scales", rows * dim // 32)
+
+
+def _vectors(n, **ts):
+    for name, t in ts.items():
+        _dense(t, name, ("torch.float32",))
+        if t.numel() < n:
+            raise MoeError("%s has %d elements, %d are needed" % (name, t.numel(), n))
+
+
+def ln_forward_act8(X, gamma, beta, Y, mean, rstd, codes, scales, fmt=ACT8_E4M3, stream=None):
+    """ln_forward that also leaves an 8-bit checkpoint of X (include/tmt_norm.h): codes rows * dim bytes, scales rows * dim / 32."""
+    lib = load()
+    if _values(X, "X") != BF16 or _values(Y, "Y") != BF16 or X.shape != Y.shape:
+        raise MoeError("X and Y must be bf16 matrices of the same shape")
+    rows, dim = X.shape
+    _vectors(dim, gamma=gamma, beta=beta)
+    _vectors(rows, mean=mean, rstd=rstd)
+    _ln_checkpoint(codes, scales, rows, dim)
+    _check(lib.tmt_ln_forward_act8(X.data_ptr(), gamma.data_ptr(), beta.data_ptr(), Y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                   codes.data_ptr(), scales.data_ptr(), fmt, rows, dim, stream), lib)
+
+
+def ln_backward_act8_scratch_bytes(rows, dim):
+    return int(load().tmt_ln_backward_act8_scratch_bytes(rows, dim))
+
+
+def ln_backward_act8(codes, scales, dY, gamma, mean, rstd, dX, dGamma, dBeta, scratch, fmt=ACT8_E4M3, stream=None):
+    """ln_backward from the checkpoint ln_forward_act8 left; scratch: ln_backward_act8_scratch_bytes(rows, dim) bytes."""
+    lib = load()
+    if _values(dY, "dY") != BF16 or _values(dX, "dX") != BF16 or dX.shape != dY.shape:
+        raise MoeError("dY and dX must be bf16 matrices of the same shape")
+    rows, dim = dY.shape
+    _vectors(dim, gamma=gamma, dGamma=dGamma, dBeta=dBeta)
+    _vectors(rows, mean=mean, rstd=rstd)
+    _ln_checkpoint(codes, scales, rows, dim)
+    _dense(scratch, "scratch", _BYTES + ("torch.float32",))
+    if scratch.numel() * scratch.element_size() < lib.tmt_ln_backward_act8_scratch_bytes(rows, dim):
+        raise MoeError("scratch is too small (ln_backward_act8_scratch_bytes)")
+    _check(lib.tmt_ln_backward_act8(codes.data_ptr(), scales.data_ptr(), fmt, dY.data_ptr(), gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                    dX.data_ptr(), dGamma.data_ptr(), dBeta.data_ptr(), rows, dim, scratch.data_ptr(), stream), lib)

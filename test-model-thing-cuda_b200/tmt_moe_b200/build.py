@@ -23,8 +23,8 @@ def _newest_source():
     
 
 def stale():
-    inc = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "tmt_moe.h")
-    newest = max(_newest_source(), os.path.getmtime(inc) if os.path.exists(inc) else 0)
+    inc = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
+    newest = max([_newest_source()] + [os.path.getmtime(os.path.join(inc, f)) for f in (os.listdir(inc) if os.path.isdir(inc) else [])])
     return not os.path.exists(LIB) or os.path.getmtime(LIB) < newest
 
 
