@@ -19,20 +19,17 @@
 #include <string>
 
 #include "launch_pdl.cuh"
-#include "mx.cuh"
-#include "mx_gemm.h"
-#include "tc_util.cuh"
+#include "mx_gemm.cuh"
 
 namespace tmt {
 namespace {
 
-using namespace tc;
-using namespace mx;
+using namespace mxg;
 
 constexpr int kBP = 128;                 // rows of a tile on the P side
-constexpr int kKB = 256;                 // elements of k per pipeline stage: one 128-byte swizzle row, two scale tiles
-constexpr int kMaxExperts = 256;
 constexpr int kThreads = 224;
+
+constexpr int kActBox = kMxActRows[kMxFew];      // few rows: activation rows per box
 
 template <int BN> struct Shape {
     static constexpr int kQBands = (BN + 127) / 128;                     // 128-row bands of scale tiles on the Q side
@@ -50,10 +47,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// 512-byte scale tile in shared memory: 32 rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle
-__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
-}
 __device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
@@ -65,78 +58,14 @@ __device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t dp, uint64_t 
         ::"r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(sfp), "r"(sfq), "r"(accumulate) : "memory");
 }
 
-struct Groups {                          // in shared memory: the experts' groups and their tiles on the activation side
-    int first[kMaxExperts + 1];          // first activation tile of each group
-    int poff[kMaxExperts], count[kMaxExperts];
-};
-struct Tile {
-    int expert, row0, rows, w0;          // activation rows [row0, row0 + rows), weight rows from w0
-};
-
-template <int TA>                        // activation rows of a tile
-__device__ __forceinline__ void load_groups(const MxGemm& p, Groups& g) {
-    if (p.experts == 0) {
-        if (threadIdx.x == 0) { g.first[0] = 0; g.first[1] = (p.rows + TA - 1) / TA; g.poff[0] = 0; g.count[0] = p.rows; }
-        return;
-    }
-    for (int e = threadIdx.x; e < p.experts; e += kThreads) {
-        const int r0 = p.poff[e];
-        int c = p.counts[e];
-        if (r0 < 0 || (r0 & 127) || c < 0 || (long)r0 + c > p.row_limit) { report(p.status, kErrSlotRange); c = 0; }
-        g.poff[e] = r0; g.count[e] = c;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {              // prefix sum over the experts, 32 at a time
-        int base = 0;
-        for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            const int e = e0 + threadIdx.x;
-            const int t = e < p.experts ? (g.count[e] + TA - 1) / TA : 0;
-            int incl = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if ((int)threadIdx.x >= o) incl += v;
-            }
-            if (e < p.experts) g.first[e] = base + incl - t;
-            base += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (threadIdx.x == 0) g.first[p.experts] = base;
-    }
-}
-template <int TA, int TW>
-__device__ __forceinline__ bool get_tile(const MxGemm& p, const Groups& g, int t, int w_tiles, Tile& ti) {
-    const int ng = p.experts == 0 ? 1 : p.experts;
-    const int at = t / w_tiles;
-    if (at >= g.first[ng]) return false;
-    int lo = 0, hi = ng;                 // last expert whose first tile is <= at and that has tiles
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (g.first[mid] <= at) lo = mid; else hi = mid; }
-    const int off = (at - g.first[lo]) * TA;
-    ti.expert = lo;
-    ti.row0 = g.poff[lo] + off;
-    ti.rows = min(TA, g.count[lo] - off);
-    ti.w0 = (t - at * w_tiles) * TW;
-    return true;
-}
-
 // ---- epilogues of one warp: its 32 TMEM lanes, all columns of the tile ----
 
-// 32 neighbouring outputs of one activation row. `word` collects the scale bytes of 4 blocks.
+// 32 neighbouring outputs of one activation row (kMxUp: after the silu). `word` collects the scale bytes of 4 blocks.
 template <int EPI>
 __device__ __forceinline__ void drain_chunk(const MxGemm& p, long row, int col0, float gate, float (&v)[32], uint32_t& word) {
     if constexpr (EPI == kMxUp) {            // one block (n is a multiple of 64 here)
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) { v[i] *= sigmoid_fast(v[i]); m = max(m, __float_as_uint(v[i]) & 0x7fffffffu); }
-        const uint32_t sb = scale_byte<kE2M1>(m);
-        const float inv = inv_scale(sb);
         uint32_t q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = v[8 * j + i] * inv;
-            q[j] = sb == 255u ? 0u : pack_e2m1x8(f);
-        }
+        const uint32_t sb = quantize32(v, q);
         stg16(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col0 / 2, make_uint4(q[0], q[1], q[2], q[3]));
         const int k4 = (col0 >> 5) & 3;
         word |= sb << (8 * k4);
@@ -178,6 +107,7 @@ __device__ __forceinline__ void drain_rows(const MxGemm& p, const Tile& ti, uint
         float v[32];
         __syncwarp();
         tmem_ld32(tm + (uint32_t)(cc * 32), v);
+        if constexpr (EPI == kMxUp) silu32(v);
         if (row_ok) drain_chunk<EPI>(p, row, col0, gate, v, word);
     }
 }
@@ -289,10 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
                     const uint32_t fb = smem_u32(&full_bar[s]);
                     const uint32_t sf_bytes = (uint32_t)min(2, tiles_k - 2 * kb) * kScaleTile;
                     if (FEW && !is_p) {                        // only the 32-row boxes that hold rows of this tile
-                        const int boxes = (ti.rows + kMxFewRows - 1) / kMxFewRows;
-                        mbar_expect_tx(fb, boxes * (kMxFewRows * 128) + sf_bytes);
+                        const int boxes = (ti.rows + kActBox - 1) / kActBox;
+                        mbar_expect_tx(fb, boxes * (kActBox * 128) + sf_bytes);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(codes_q + s * S::kCodesQ + b * (kMxFewRows * 128), map, fb, kb * 128, row + b * kMxFewRows);
+                            tma_load_2d(codes_q + s * S::kCodesQ + b * (kActBox * 128), map, fb, kb * 128, row + b * kActBox);
                     } else {
                         mbar_expect_tx(fb, (is_p ? S::kCodesP : S::kCodesQ) + bands * sf_bytes);
                         tma_load_2d(is_p ? codes_p + s * S::kCodesP : codes_q + s * S::kCodesQ, map, fb, kb * 128, row);
@@ -315,8 +245,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
         __syncwarp();
     } else if (warp == 1) {
         // ---------------- MMA issuer: the whole warp runs the loop, one elected lane issues ----------------
-        // e2m1 operands, e8m0 scales, both K-major; the scale ids (0 or 2) pick the blocks 0-1 or 2-3 of a tile
-        const uint32_t idesc_mn = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kBP >> 4) << 24);
         const uint32_t sfp_t = tmem_base + S::kSfCol, sfq_t = sfp_t + 8;
         int s = 0; uint32_t ph = 0;
         int acc = 0; uint32_t acc_ph = 0;
@@ -330,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
             const uint32_t d_tmem = tmem_base + acc * BN;
             // few rows: as many columns as the tile has rows. A tile starts on a 128-row band of scales, so the scale columns of
             // an MMA always start on a whole tile's first column (a start inside a tile is not a form this kernel relies on).
-            const uint32_t cols_q = FEW ? (uint32_t)((ti.rows + kMxFewRows - 1) / kMxFewRows * kMxFewRows) : (uint32_t)BN;
-            const uint32_t idesc0 = idesc_mn | ((cols_q >> 3) << 17);
+            const uint32_t cols_q = FEW ? (uint32_t)((ti.rows + kActBox - 1) / kActBox * kActBox) : (uint32_t)BN;
+            const uint32_t idesc0 = mxf4_idesc(kBP, cols_q);
             for (int kb = 0; kb < nkb; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, p.status));
                 if (!ok) break;
@@ -351,8 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (j < steps) {
-                            const uint32_t id = (j & 1) * 2;
-                            mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | (id << 4) | (id << 29), sfp_t + (j >> 1) * 4,
+                                                        mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | mxf4_ids((j & 1) * 2), sfp_t + (j >> 1) * 4,
                                      sfq_t + (j >> 1) * 4 * S::kQBands, (kb | j) != 0);
                         }
                     tc_commit(smem_u32(&empty_bar[s]));
@@ -427,21 +354,46 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-bool mx_few_rows(long rows_per_group) { return rows_per_group <= 32; }
+int mx_form(long rows, int groups, int n, int num_sms, int pad) {
+    const long each = (rows + groups - 1) / groups;
+    if (each <= 32) return kMxFew;
+    const long pairs = groups * ((each + 255) / 256) * ((n + 255) / 256);
+    return pad % 256 == 0 && pairs >= num_sms / 2 ? kMxPair : kMxMany;
+}
+
+namespace {
+void encode(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion l2) {
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode_fn()(m, type, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, l2,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed for a 4-bit product (" + std::to_string((int)r) + ")");
+}
+}  // namespace
 
 void mx_make_map(CUtensorMap* m, const void* codes, uint64_t rows, int cols, int box_rows) {
-    const cuuint64_t dims[2] = {(cuuint64_t)cols / 2, rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)cols / 2};
+    const cuuint64_t dims[2] = {(cuuint64_t)cols / 2, rows}, strides[1] = {(cuuint64_t)cols / 2};
     const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
-                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed for a 4-bit matrix (" + std::to_string((int)r) + ")");
+    encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+void mx_make_scale_map(CUtensorMap* m, const void* scales, uint64_t rows, int cols, int bands) {
+    const cuuint64_t tiles_k = (cuuint64_t)scale_tiles_k(cols);
+    const cuuint64_t dims[3] = {kScaleTile / 4, tiles_k, (rows + 127) / 128}, strides[2] = {kScaleTile, tiles_k * kScaleTile};
+    const cuuint32_t box[3] = {kScaleTile / 4, 2u, (cuuint32_t)bands};
+    encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+void mx_make_out_map(CUtensorMap* m, void* out, uint64_t rows, int n, bool f32) {
+    const cuuint64_t dims[2] = {(cuuint64_t)n, rows}, strides[1] = {(cuuint64_t)n * (f32 ? 4 : 2)};
+    const cuuint32_t box[2] = {f32 ? 32u : 64u, 32u};
+    encode(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 cudaError_t launch_mx_gemm(const MxGemm& p, int num_sms, cudaStream_t stream) {
-    return p.few_rows ? launch_epi<128, true>(p, num_sms, stream) : launch_epi<128, false>(p, num_sms, stream);
+    if (p.form == kMxPair) return launch_mx_gemm_2cta(p, num_sms, stream);
+    return p.form == kMxFew ? launch_epi<128, true>(p, num_sms, stream) : launch_epi<128, false>(p, num_sms, stream);
 }
 
 }  // namespace tmt

@@ -1,0 +1,122 @@
+// Device pieces shared by the two 4-bit product kernels (mx_gemm.cu, mx_gemm_2cta.cu): descriptors, groups and tiles.
+#pragma once
+#include "mx.cuh"
+#include "mx_gemm.h"
+#include "tc_util.cuh"
+
+namespace tmt {
+namespace mxg {
+
+using namespace tc;
+using namespace mx;
+
+constexpr int kKB = 256;                 // elements of k per pipeline stage: one 128-byte swizzle row, two scale tiles
+constexpr int kMaxExperts = 256;
+
+// Instruction descriptor: e2m1 operands, e8m0 scales, both K-major, m rows x n columns. The scale ids (0 or 2) pick the
+// blocks 0-1 or 2-3 of a scale tile, i.e. the first or second 64 elements of its 128.
+__device__ __forceinline__ uint32_t mxf4_idesc(uint32_t m, uint32_t n) { return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24); }
+__device__ __forceinline__ uint32_t mxf4_ids(uint32_t id) { return (id << 4) | (id << 29); }
+// 512-byte scale tile in shared memory: 32 rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
+}
+struct Groups {                          // in shared memory: the experts' groups and their tiles on the activation side
+    int first[kMaxExperts + 1];          // first activation tile of each group
+    int poff[kMaxExperts], count[kMaxExperts];
+};
+struct Tile {
+    int expert, row0, rows, w0;          // activation rows [row0, row0 + rows), weight rows from w0
+};
+
+template <int TA>                        // activation rows of a tile
+__device__ __forceinline__ void load_groups(const MxGemm& p, Groups& g) {
+    if (p.experts == 0) {
+        if (threadIdx.x == 0) { g.first[0] = 0; g.first[1] = (p.rows + TA - 1) / TA; g.poff[0] = 0; g.count[0] = p.rows; }
+        return;
+    }
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
+        const int r0 = p.poff[e];
+        int c = p.counts[e];
+        if (r0 < 0 || (r0 & 127) || c < 0 || (long)r0 + c > p.row_limit) { report(p.status, kErrSlotRange); c = 0; }
+        g.poff[e] = r0; g.count[e] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {              // prefix sum over the experts, 32 at a time
+        int base = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + threadIdx.x;
+            const int t = e < p.experts ? (g.count[e] + TA - 1) / TA : 0;
+            int incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if ((int)threadIdx.x >= o) incl += v;
+            }
+            if (e < p.experts) g.first[e] = base + incl - t;
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (threadIdx.x == 0) g.first[p.experts] = base;
+    }
+}
+template <int TA, int TW>
+__device__ __forceinline__ bool get_tile(const MxGemm& p, const Groups& g, int t, int w_tiles, Tile& ti) {
+    const int ng = p.experts == 0 ? 1 : p.experts;
+    const int at = t / w_tiles;
+    if (at >= g.first[ng]) return false;
+    int lo = 0, hi = ng;                 // last expert whose first tile is <= at and that has tiles
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (g.first[mid] <= at) lo = mid; else hi = mid; }
+    const int off = (at - g.first[lo]) * TA;
+    ti.expert = lo;
+    ti.row0 = g.poff[lo] + off;
+    ti.rows = min(TA, g.count[lo] - off);
+    ti.w0 = (t - at * w_tiles) * TW;
+    return true;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp_fast(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// silu of 32 accumulators, in place. The special-function unit sets the pace of this epilogue (16 results a clock and SM): two
+// elements share one reciprocal, 1 / a = b / (a b), so that an element costs 1.5 of its results instead of 2. a b stays finite,
+// and its reciprocal a normal number, while both exponents are below 43; a warp that holds an element below -43 takes the plain form.
+__device__ __forceinline__ void silu32(float (&f)[32]) {
+    float lo = fminf(f[0], f[1]);
+#pragma unroll
+    for (int i = 2; i < 32; i += 2) lo = fminf(fminf(lo, f[i]), f[i + 1]);
+    if (__all_sync(0xffffffffu, lo > -43.0f)) {          // false for a NaN in every element alone; others propagate through either form
+        const float2 c = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.0f, 1.0f);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 x = make_float2(f[i], f[i + 1]);
+            float2 e = __fmul2_rn(x, c);
+            e = __fadd2_rn(make_float2(exp2_fast(e.x), exp2_fast(e.y)), one);
+            const float r = rcp_fast(e.x * e.y);
+            f[i] = x.x * (r * e.y);
+            f[i + 1] = x.y * (r * e.x);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = f[i] * sigmoid_fast(f[i]);
+    }
+}
+// One block of 32 -> its 4-bit codes, element 0 in the lowest nibble of q[0]; returns the scale byte.
+__device__ __forceinline__ uint32_t quantize32(const float (&f)[32], uint32_t (&q)[4]) {
+    float m = 0.0f;                                      // NaN-propagating maximum of the magnitudes
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+        asm("{\n\t.reg .f32 a, b;\n\tabs.f32 a, %1;\n\tabs.f32 b, %2;\n\tmax.NaN.f32 a, a, b;\n\tmax.NaN.f32 %0, %0, a;\n\t}" : "+f"(m) : "f"(f[i]), "f"(f[i + 1]));
+    const uint32_t sb = scale_byte<kE2M1>(__float_as_uint(m));
+    const float inv = inv_scale(sb);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = f[8 * j + i] * inv;
+        q[j] = sb == 255u ? 0u : pack_e2m1x8(g);
+    }
+    return sb;
+}
+
+}  // namespace mxg
+}  // namespace tmt

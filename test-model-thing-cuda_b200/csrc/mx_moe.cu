@@ -89,6 +89,9 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
     }
 }
 
+// Per-expert maps: of each product the codes in boxes of 128 rows, in boxes of 64 (pair form), and the scale tiles (pair form).
+enum Table : int { kTabCodes = 0, kTabCodesPair, kTabScales, kTabsPerProduct, kTables = 2 * kTabsPerProduct };
+
 template <class T>
 T* alloc(tmt_moe* h, size_t n) {
     void* p = nullptr;
@@ -107,14 +110,17 @@ void make_buffers(tmt_moe* h) {
     m.x_scales = alloc<uint8_t>(h, scale_bytes(cap, D));
     m.h_codes = alloc<uint8_t>(h, (size_t)cap * H / 2);
     m.h_scales = alloc<uint8_t>(h, scale_bytes(cap, H));
-    for (int few = 0; few < 2; ++few) {
-        mx_make_map(&m.x_map[few], m.x_codes, cap, D, few ? kMxFewRows : kMxMapRows);
-        mx_make_map(&m.h_map[few], m.h_codes, cap, H, few ? kMxFewRows : kMxMapRows);
+    for (int f = 0; f < kMxForms; ++f) {
+        mx_make_map(&m.x_map[f], m.x_codes, cap, D, kMxActRows[f]);
+        mx_make_map(&m.h_map[f], m.h_codes, cap, H, kMxActRows[f]);
     }
+    mx_make_scale_map(&m.x_sf, m.x_scales, cap, D, kMxActBands);
+    mx_make_scale_map(&m.h_sf, m.h_scales, cap, H, kMxActBands);
+    mx_make_out_map(&m.y_out, h->Yg, cap, D, false);
     // the padding rows' scale bytes are read with the others (their products are never used): give them a value
     cuda_ok(cudaMemsetAsync(m.x_scales, 0, scale_bytes(cap, D), h->stream), "cudaMemsetAsync");
     cuda_ok(cudaMemsetAsync(m.h_scales, 0, scale_bytes(cap, H), h->stream), "cudaMemsetAsync");
-    m.tables = alloc<CUtensorMap>(h, 2 * (size_t)E);
+    m.tables = alloc<CUtensorMap>(h, kTables * (size_t)E);
     m.scale_tab = alloc<const uint8_t*>(h, 2 * (size_t)E);
 }
 
@@ -127,11 +133,15 @@ void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_wei
     if (key == m.key) return;
     m.key.clear();                       // stays empty if anything below throws
     for (const void* p : key) check_tensors({p});
-    std::vector<CUtensorMap> maps(2 * (size_t)E);
-    for (int e = 0; e < E; ++e) {
-        mx_make_map(&maps[e], Wup[e].codes, Wup[e].rows, Wup[e].cols, kMxMapRows);
-        mx_make_map(&maps[E + e], Wdown[e].codes, Wdown[e].rows, Wdown[e].cols, kMxMapRows);
-    }
+    std::vector<CUtensorMap> maps(kTables * (size_t)E);
+    for (int product = 0; product < 2; ++product)
+        for (int e = 0; e < E; ++e) {
+            const tmt_mxfp4_weight& w = product == 0 ? Wup[e] : Wdown[e];
+            CUtensorMap* t = maps.data() + (size_t)product * kTabsPerProduct * E + e;
+            mx_make_map(t + (size_t)kTabCodes * E, w.codes, w.rows, w.cols, kMxWeightRows[kMxMany]);
+            mx_make_map(t + (size_t)kTabCodesPair * E, w.codes, w.rows, w.cols, kMxWeightRows[kMxPair]);
+            mx_make_scale_map(t + (size_t)kTabScales * E, w.scales, w.rows, w.cols, kMxWeightBands);
+        }
     cuda_ok(cudaMemcpyAsync(m.tables, maps.data(), maps.size() * sizeof(CUtensorMap), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
     cuda_ok(cudaMemcpyAsync(m.scale_tab, key.data(), 2 * (size_t)E * sizeof(void*), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
     cuda_ok(cudaStreamSynchronize(h->stream), "cudaStreamSynchronize");      // the host vectors are about to go
@@ -161,15 +171,23 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     memset(&p, 0, sizeof p);
     p.experts = E; p.poff = h->rb.poff; p.counts = h->rb.counts; p.row_limit = h->dims.cap;
     p.status = h->rb.status;
-    p.few_rows = mx_few_rows(((long)tokens * K + E - 1) / E);
-    p.act = m.x_map[p.few_rows]; p.act_scales = m.x_scales;
-    p.w_maps = m.tables; p.w_scales_tab = m.scale_tab;
+    // a product's view of the per-expert tables
+    auto weights = [&](int product) {
+        const CUtensorMap* t = m.tables + (size_t)product * kTabsPerProduct * E;
+        p.w_maps = t + (size_t)(p.form == kMxPair ? kTabCodesPair : kTabCodes) * E;
+        p.w_sf_maps = t + (size_t)kTabScales * E;
+        p.w_scales_tab = m.scale_tab + (size_t)product * E;
+    };
     p.n = H; p.k = D; p.epi = kMxUp; p.out = m.h_codes; p.out_scales = m.h_scales;
+    p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
+    p.act = m.x_map[p.form]; p.act_scales = m.x_scales; p.act_sf = m.x_sf;
+    weights(0);
     prof_mark(h, kPhGemmUp);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
-    p.act = m.h_map[p.few_rows]; p.act_scales = m.h_scales;
-    p.w_maps = m.tables + E; p.w_scales_tab = m.scale_tab + E;
-    p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.row_scale = h->rb.slotw;
+    p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
+    p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
+    p.act = m.h_map[p.form]; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
+    weights(1);
     prof_mark(h, kPhGemmDown);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx down launch");
     prof_mark(h, kPhCombine);
@@ -188,13 +206,19 @@ void check_weight(const tmt_mxfp4_weight* W) {
 void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
     MxGemm p;
     memset(&p, 0, sizeof p);
-    p.few_rows = mx_few_rows(rows);
-    mx_make_map(&p.act, codes, rows, W.cols, p.few_rows ? kMxFewRows : kMxMapRows);
-    mx_make_map(&p.w, W.codes, W.rows, W.cols, kMxMapRows);
-    p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
+    const int sms = sm_count();
     p.rows = rows; p.n = W.rows; p.k = W.cols;
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
-    cuda_ok(launch_mx_gemm(p, sm_count(), s), "matmul_mxfp4 launch");
+    p.form = mx_form(rows, 1, p.n, sms, 256);
+    p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
+    mx_make_map(&p.act, codes, rows, p.k, kMxActRows[p.form]);
+    mx_make_map(&p.w, W.codes, p.n, p.k, kMxWeightRows[p.form]);
+    if (p.form == kMxPair) {
+        mx_make_scale_map(&p.act_sf, scales, rows, p.k, kMxActBands);
+        mx_make_scale_map(&p.w_sf, W.scales, p.n, p.k, kMxWeightBands);
+        mx_make_out_map(&p.out_map, Y, rows, p.n, p.epi == kMxF32);
+    }
+    cuda_ok(launch_mx_gemm(p, sms, s), "matmul_mxfp4 launch");
 }
 
 void check_dtype(int dtype) {
