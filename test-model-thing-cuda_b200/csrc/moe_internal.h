@@ -34,8 +34,7 @@ struct Profiler {
 // blocks, and the per-expert tables of the weights last handed in.
 struct MxState {
     uint8_t *x_codes = nullptr, *x_scales = nullptr, *h_codes = nullptr, *h_scales = nullptr;
-    CUtensorMap x_map[kMxForms] = {}, h_map[kMxForms] = {};      // codes, by form of the product
-    CUtensorMap x_sf = {}, h_sf = {}, y_out = {};
+    CUtensorMap x_map = {}, h_map = {}, x_sf = {}, h_sf = {}, y_out = {};
     CUtensorMap* tables = nullptr;                 // per-expert weight maps (mx_moe.cu)
     const uint8_t** scale_tab = nullptr;           // [2][E]
     std::vector<const void*> key;                  // the pointers the tables were built from

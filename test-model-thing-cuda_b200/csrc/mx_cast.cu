@@ -57,8 +57,8 @@ __device__ __forceinline__ uint32_t spread8(const Vec8<F32>& v, float (&f)[8]) {
 template <int FMT, bool F32, int U>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __restrict__ X, unsigned rows, int cols, unsigned chunks,
                                                                unsigned per_row, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, bool early) {
-    if (early) pdl_begin();
     pdl_wait();
+    if (early) pdl_begin();
     const int lane = threadIdx.x & 31;
     const unsigned c0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * U;
     const unsigned full = 0xffffffffu;

@@ -3,9 +3,7 @@
 //
 //   acc[i, j] = sum over blocks b of  sP[i, b] sQ[j, b]  sum over the block of qP qQ
 //
-// P is the operand on the 128-row side of the MMA, Q the one on its column side. Many rows: P = activations, Q = weights.
-// Few rows (a decode step): P = weights, Q = activations, so that a tile is 128 weight rows x the rows there are (in steps of 32,
-// up to 128) instead of 128 mostly empty rows, and the call is bound by streaming the weights once.
+// Operand P, on the 128-row side of the MMA, are activations, Q, on its column side, weights.
 //
 // Codes travel by TMA in boxes of 128 bytes (256 elements of k) with the 128-byte swizzle, exactly as a bf16 operand of 64
 // elements would; an MMA takes 64 elements (32 bytes). Scales travel as whole 512-byte tiles (128 rows x 4 blocks) by untiled
@@ -28,8 +26,6 @@ using namespace mxg;
 
 constexpr int kBP = 128;                 // rows of a tile on the P side
 constexpr int kThreads = 224;
-
-constexpr int kActBox = kMxActRows[kMxFew];      // few rows: activation rows per box
 
 template <int BN> struct Shape {
     static constexpr int kQBands = (BN + 127) / 128;                     // 128-row bands of scale tiles on the Q side
@@ -112,48 +108,10 @@ __device__ __forceinline__ void drain_rows(const MxGemm& p, const Tile& ti, uint
     }
 }
 
-// Few rows: lane = output (a weight row), columns = activation rows.
-template <int EPI, int BN>
-__device__ __forceinline__ void drain_cols(const MxGemm& p, const Tile& ti, uint32_t tm, int o, int lane) {
-    const int col = ti.w0 + o;
-    const bool col_ok = col < p.n;
-    const unsigned full = 0xffffffffu;
-#pragma unroll 1
-    for (int cc = 0; cc < BN / 32; ++cc) {
-        if (cc * 32 >= ti.rows) break;
-        float v[32];
-        tmem_ld32(tm + (uint32_t)(cc * 32), v);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if (cc * 32 + i >= ti.rows) break;
-            const long row = (long)ti.row0 + cc * 32 + i;
-            if constexpr (EPI == kMxUp) {        // the warp's 32 outputs are one block (col - lane is a multiple of 32)
-                const float s = v[i] * sigmoid_fast(v[i]);
-                const uint32_t m = __reduce_max_sync(full, __float_as_uint(s) & 0x7fffffffu);
-                const uint32_t sb = scale_byte<kE2M1>(m);
-                float f[8] = {s * inv_scale(sb), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t q = sb == 255u ? 0u : (pack_e2m1x8(f) & 15u) << (4 * (lane & 7));
-                q |= __shfl_xor_sync(full, q, 1);
-                q |= __shfl_xor_sync(full, q, 2);
-                q |= __shfl_xor_sync(full, q, 4);
-                if (col_ok) {
-                    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col / 2) = q;
-                    if (lane == 0) p.out_scales[scale_word(row, col >> 7, scale_tiles_k(p.n)) + ((col >> 5) & 3)] = (uint8_t)sb;
-                }
-            } else if constexpr (EPI == kMxF32) {
-                if (col_ok) static_cast<float*>(p.out)[row * p.n + col] = v[i];
-            } else {
-                const float x = EPI == kMxDown ? v[i] * __ldg(p.row_scale + row) : v[i];
-                if (col_ok) static_cast<uint16_t*>(p.out)[row * p.n + col] = f2bf(x);
-            }
-        }
-    }
-}
-
-template <int BN, bool FEW, int EPI>
+template <int BN, int EPI>
 __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_constant__ MxGemm p) {
     using S = Shape<BN>;
-    constexpr int TA = FEW ? BN : kBP, TW = FEW ? kBP : BN;       // activation / weight rows of a tile
+    constexpr int TA = kBP, TW = BN;       // activation / weight rows of a tile
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[S::kStages], empty_bar[S::kStages], tfull_bar[2], tempty_bar[2];
     __shared__ Groups groups;
@@ -191,7 +149,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
         // ---------------- producers: codes box and scale tiles of one operand per stage ----------------
         if (lane == 0) {
             const bool is_p = warp == 0;
-            const bool is_act = is_p != FEW;
             int s = 0; uint32_t ph = 0;
             uint32_t issued = 0, last_parity = 0;
             bool ok = true;
@@ -203,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
                 int row;
                 long band;                                     // first 128-row band of scale tiles
                 int bands = 1;
-                if (is_act) {
+                if (is_p) {
                     map = &p.act; sc = p.act_scales; row = ti.row0;
                 } else {
                     map = p.w_maps ? p.w_maps + ti.expert : &p.w;
@@ -212,21 +169,14 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
                     if (p.w_maps) tensormap_acquire(map);
                 }
                 band = row >> 7;
-                if (!is_p) bands = min(S::kQBands, is_act ? 1 : (p.n - row + 127) / 128);
+                if (!is_p) bands = min(S::kQBands, (p.n - row + 127) / 128);
                 for (int kb = 0; kb < nkb; ++kb) {
                     ok = mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, p.status);
                     if (!ok) break;
                     const uint32_t fb = smem_u32(&full_bar[s]);
                     const uint32_t sf_bytes = (uint32_t)min(2, tiles_k - 2 * kb) * kScaleTile;
-                    if (FEW && !is_p) {                        // only the 32-row boxes that hold rows of this tile
-                        const int boxes = (ti.rows + kActBox - 1) / kActBox;
-                        mbar_expect_tx(fb, boxes * (kActBox * 128) + sf_bytes);
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(codes_q + s * S::kCodesQ + b * (kActBox * 128), map, fb, kb * 128, row + b * kActBox);
-                    } else {
-                        mbar_expect_tx(fb, (is_p ? S::kCodesP : S::kCodesQ) + bands * sf_bytes);
-                        tma_load_2d(is_p ? codes_p + s * S::kCodesP : codes_q + s * S::kCodesQ, map, fb, kb * 128, row);
-                    }
+                    mbar_expect_tx(fb, (is_p ? S::kCodesP : S::kCodesQ) + bands * sf_bytes);
+                    tma_load_2d(is_p ? codes_p + s * S::kCodesP : codes_q + s * S::kCodesQ, map, fb, kb * 128, row);
                     const uint32_t sf = is_p ? sf_p + s * S::kSfP : sf_q + s * S::kSfQ;
                     for (int b = 0; b < bands; ++b)
                         bulk_load(sf + b * 2 * kScaleTile, sc + ((size_t)(band + b) * tiles_k + 2 * kb) * kScaleTile, sf_bytes, fb);
@@ -246,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     } else if (warp == 1) {
         // ---------------- MMA issuer: the whole warp runs the loop, one elected lane issues ----------------
         const uint32_t sfp_t = tmem_base + S::kSfCol, sfq_t = sfp_t + 8;
+        const uint32_t idesc0 = mxf4_idesc(kBP, BN);
         int s = 0; uint32_t ph = 0;
         int acc = 0; uint32_t acc_ph = 0;
         bool ok = true;
@@ -256,10 +207,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
             if (!ok) break;
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * BN;
-            // few rows: as many columns as the tile has rows. A tile starts on a 128-row band of scales, so the scale columns of
-            // an MMA always start on a whole tile's first column (a start inside a tile is not a form this kernel relies on).
-            const uint32_t cols_q = FEW ? (uint32_t)((ti.rows + kActBox - 1) / kActBox * kActBox) : (uint32_t)BN;
-            const uint32_t idesc0 = mxf4_idesc(kBP, cols_q);
             for (int kb = 0; kb < nkb; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, p.status));
                 if (!ok) break;
@@ -303,8 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[acc]), acc_ph, abort_flag, p.status))) break;
             tc_fence_after();
             const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
-            if constexpr (FEW) drain_cols<EPI, BN>(p, ti, tm, quarter * 32 + lane, lane);
-            else drain_rows<EPI, BN>(p, ti, tm, quarter * 32 + lane);
+            drain_rows<EPI, BN>(p, ti, tm, quarter * 32 + lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
@@ -319,20 +265,20 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     }
 }
 
-template <int BN, bool FEW, int EPI>
+template <int BN, int EPI>
 cudaError_t launch_t(const MxGemm& p, int grid, cudaStream_t stream) {
     constexpr int smem = Shape<BN>::kSmem;
-    const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<BN, FEW, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(mx_gemm_kernel<BN, FEW, EPI>, dim3(grid), dim3(kThreads), smem, stream, p);
+    return launch_pdl(mx_gemm_kernel<BN, EPI>, dim3(grid), dim3(kThreads), smem, stream, p);
 }
-template <int BN, bool FEW>
+template <int BN>
 cudaError_t launch_epi(const MxGemm& p, int grid, cudaStream_t stream) {
     switch (p.epi) {
-        case kMxBf16: return launch_t<BN, FEW, kMxBf16>(p, grid, stream);
-        case kMxF32: return launch_t<BN, FEW, kMxF32>(p, grid, stream);
-        case kMxUp: return launch_t<BN, FEW, kMxUp>(p, grid, stream);
-        case kMxDown: return launch_t<BN, FEW, kMxDown>(p, grid, stream);
+        case kMxBf16: return launch_t<BN, kMxBf16>(p, grid, stream);
+        case kMxF32: return launch_t<BN, kMxF32>(p, grid, stream);
+        case kMxUp: return launch_t<BN, kMxUp>(p, grid, stream);
+        case kMxDown: return launch_t<BN, kMxDown>(p, grid, stream);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -356,7 +302,6 @@ EncodeTiledFn encode_fn() {
 
 int mx_form(long rows, int groups, int n, int num_sms, int pad) {
     const long each = (rows + groups - 1) / groups;
-    if (each <= 32) return kMxFew;
     const long pairs = groups * ((each + 255) / 256) * ((n + 255) / 256);
     return pad % 256 == 0 && pairs >= num_sms / 2 ? kMxPair : kMxMany;
 }
@@ -393,7 +338,7 @@ void mx_make_out_map(CUtensorMap* m, void* out, uint64_t rows, int n, bool f32) 
 
 cudaError_t launch_mx_gemm(const MxGemm& p, int num_sms, cudaStream_t stream) {
     if (p.form == kMxPair) return launch_mx_gemm_2cta(p, num_sms, stream);
-    return p.form == kMxFew ? launch_epi<128, true>(p, num_sms, stream) : launch_epi<128, false>(p, num_sms, stream);
+    return launch_epi<128>(p, num_sms, stream);
 }
 
 }  // namespace tmt

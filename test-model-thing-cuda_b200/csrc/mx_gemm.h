@@ -19,7 +19,7 @@ struct MxGemm {
     CUtensorMap act, w;                 // codes as bytes, 128-byte boxes (mx_act_map / mx_weight_map)
     const CUtensorMap* w_maps;          // grouped: one map per expert in device memory (then `w` is not used)
     // scale tiles of the activations (group starts are multiples of 128 rows, of 256 for kMxPair) and of the weights
-    const uint8_t* act_scales;          // kMxMany, kMxFew
+    const uint8_t* act_scales;          // kMxMany
     const uint8_t* w_scales;            // dense
     const uint8_t* const* w_scales_tab; // grouped: per expert, device table
     CUtensorMap act_sf, w_sf;           // kMxPair: the same as 3-D maps {tile of 512 bytes, tiles along k, 128-row bands}
@@ -36,15 +36,13 @@ struct MxGemm {
     int form;                           // MxForm
 };
 
-// Forms of the product: weights on the 128-row side of the MMA; activations there, one CTA per 128 x 128 tile; CTA pairs on
-// 256 x 256 tiles.
-enum MxForm : int { kMxFew = 0, kMxMany = 1, kMxPair = 2, kMxForms = 3 };
+// Forms of the product: one CTA per 128 x 128 tile; CTA pairs on 256 x 256 tiles.
+enum MxForm : int { kMxMany = 0, kMxPair = 1 };
 // The form for `rows` activation rows in `groups` groups of about equal size, n outputs; pad: rows that group starts are multiples of.
 int mx_form(long rows, int groups, int n, int num_sms, int pad);
 
-// Rows per box of the codes' maps by form.
-constexpr int kMxActRows[kMxForms] = {32, 128, 128};
-constexpr int kMxWeightRows[kMxForms] = {128, 128, 128};
+// 128-row boxes for the codes of both operands; 128-row bands per box of the scale maps (pair form).
+constexpr int kMxBoxRows = 128;
 constexpr int kMxActBands = 1, kMxWeightBands = 2;      // 128-row bands per box of the scale maps
 
 // 2-D byte map {cols / 2, rows} with boxes of 128 bytes x box_rows, 128-byte swizzle, zero fill.

@@ -10,8 +10,10 @@
 #include "moe_internal.h"
 #include "mx.cuh"
 #include "mx_cast.h"
+#include "mx_decode.h"
 #include "mx_gemm.h"
 #include "mx_host.h"
+#include "nvfp4_decode.h"
 
 namespace tmt {
 namespace {
@@ -89,8 +91,8 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
     }
 }
 
-// Per-expert maps: of each product the codes in boxes of 128 rows, in boxes of 64 (pair form), and the scale tiles (pair form).
-enum Table : int { kTabCodes = 0, kTabCodesPair, kTabScales, kTabsPerProduct, kTables = 2 * kTabsPerProduct };
+// Per-expert maps: of each product the codes, and the scale tiles in boxes of one band (decode form) and of two (pair form).
+enum Table : int { kTabCodes = 0, kTabScales1, kTabScales2, kTabsPerProduct, kTables = 2 * kTabsPerProduct };
 
 template <class T>
 T* alloc(tmt_moe* h, size_t n) {
@@ -110,10 +112,8 @@ void make_buffers(tmt_moe* h) {
     m.x_scales = alloc<uint8_t>(h, scale_bytes(cap, D));
     m.h_codes = alloc<uint8_t>(h, (size_t)cap * H / 2);
     m.h_scales = alloc<uint8_t>(h, scale_bytes(cap, H));
-    for (int f = 0; f < kMxForms; ++f) {
-        mx_make_map(&m.x_map[f], m.x_codes, cap, D, kMxActRows[f]);
-        mx_make_map(&m.h_map[f], m.h_codes, cap, H, kMxActRows[f]);
-    }
+    mx_make_map(&m.x_map, m.x_codes, cap, D, kMxBoxRows);
+    mx_make_map(&m.h_map, m.h_codes, cap, H, kMxBoxRows);
     mx_make_scale_map(&m.x_sf, m.x_scales, cap, D, kMxActBands);
     mx_make_scale_map(&m.h_sf, m.h_scales, cap, H, kMxActBands);
     mx_make_out_map(&m.y_out, h->Yg, cap, D, false);
@@ -138,9 +138,9 @@ void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_wei
         for (int e = 0; e < E; ++e) {
             const tmt_mxfp4_weight& w = product == 0 ? Wup[e] : Wdown[e];
             CUtensorMap* t = maps.data() + (size_t)product * kTabsPerProduct * E + e;
-            mx_make_map(t + (size_t)kTabCodes * E, w.codes, w.rows, w.cols, kMxWeightRows[kMxMany]);
-            mx_make_map(t + (size_t)kTabCodesPair * E, w.codes, w.rows, w.cols, kMxWeightRows[kMxPair]);
-            mx_make_scale_map(t + (size_t)kTabScales * E, w.scales, w.rows, w.cols, kMxWeightBands);
+            mx_make_map(t + (size_t)kTabCodes * E, w.codes, w.rows, w.cols, kMxBoxRows);
+            mx_make_scale_map(t + (size_t)kTabScales1 * E, w.scales, w.rows, w.cols, 1);
+            mx_make_scale_map(t + (size_t)kTabScales2 * E, w.scales, w.rows, w.cols, kMxWeightBands);
         }
     cuda_ok(cudaMemcpyAsync(m.tables, maps.data(), maps.size() * sizeof(CUtensorMap), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
     cuda_ok(cudaMemcpyAsync(m.scale_tab, key.data(), 2 * (size_t)E * sizeof(void*), cudaMemcpyHostToDevice, h->stream), "cudaMemcpyAsync");
@@ -164,6 +164,28 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     h->dims.T = tokens;
     h->last_tokens = tokens;
     route_only(h, static_cast<const uint16_t*>(X), Wr);
+    if (mx_decode_form((long)tokens * K, E, std::max(D, H))) {
+        // Few rows per expert: no dispatch; up finds and quantises its rows itself and writes one row per assignment, down reads those.
+        MxDecode q;
+        memset(&q, 0, sizeof q);
+        q.idx = h->rb.idx; q.n_asg = tokens * K; q.experts = E; q.status = h->rb.status; q.early = true;
+        q.src = X; q.src_kind = kMxSrcBf16; q.src_mul = mx_row_factor(K);
+        q.w_maps = m.tables + (size_t)kTabCodes * E; q.w_sf_maps = m.tables + (size_t)kTabScales1 * E;
+        q.n = H; q.k = D; q.epi = kMxUp; q.out = m.h_codes; q.out_scales = m.h_scales;
+        prof_mark(h, kPhGemmUp);
+        cuda_ok(launch_mx_decode(q, h->stream), "mx up launch");
+        q.src = m.h_codes; q.src_scales = m.h_scales; q.src_kind = kMxSrcRows; q.src_mul = mx_row_factor(1);
+        q.w_maps += (size_t)kTabsPerProduct * E; q.w_sf_maps += (size_t)kTabsPerProduct * E;
+        q.n = D; q.k = H; q.epi = kMxDown; q.out = h->Yg; q.out_scales = nullptr; q.gate = h->rb.w;
+        prof_mark(h, kPhGemmDown);
+        cuda_ok(launch_mx_decode(q, h->stream), "mx down launch");
+        prof_mark(h, kPhCombine);
+        cuda_ok(launch_decode_combine(h->Yg, static_cast<uint16_t*>(Y), beta, tokens, D, K, h->stream), "combine launch");
+        prof_mark(h, -1);
+        h->launches += 3;
+        h->have_forward = true;
+        return;
+    }
     prof_mark(h, kPhDispatch);
     cuda_ok(launch_pdl(mx_dispatch_kernel, dim3((tokens + kDispatchWarps - 1) / kDispatchWarps), dim3(kDispatchWarps * 32), E * sizeof(int),
                        h->stream, h->dims, h->rb, static_cast<const uint16_t*>(X), m.x_codes, m.x_scales), "mx dispatch launch");
@@ -174,19 +196,19 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     // a product's view of the per-expert tables
     auto weights = [&](int product) {
         const CUtensorMap* t = m.tables + (size_t)product * kTabsPerProduct * E;
-        p.w_maps = t + (size_t)(p.form == kMxPair ? kTabCodesPair : kTabCodes) * E;
-        p.w_sf_maps = t + (size_t)kTabScales * E;
+        p.w_maps = t + (size_t)kTabCodes * E;
+        p.w_sf_maps = t + (size_t)kTabScales2 * E;
         p.w_scales_tab = m.scale_tab + (size_t)product * E;
     };
     p.n = H; p.k = D; p.epi = kMxUp; p.out = m.h_codes; p.out_scales = m.h_scales;
     p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
-    p.act = m.x_map[p.form]; p.act_scales = m.x_scales; p.act_sf = m.x_sf;
+    p.act = m.x_map; p.act_scales = m.x_scales; p.act_sf = m.x_sf;
     weights(0);
     prof_mark(h, kPhGemmUp);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
     p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
     p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
-    p.act = m.h_map[p.form]; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
+    p.act = m.h_map; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
     weights(1);
     prof_mark(h, kPhGemmDown);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx down launch");
@@ -203,7 +225,20 @@ void check_weight(const tmt_mxfp4_weight* W) {
         throw std::runtime_error("MXFP4 weight: rows must be a positive multiple of 8, cols of 64");
 }
 
+// Up to 32 rows, from values or from codes.
+void few_rows(const void* src, const void* scales, int kind, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
+    MxDecode p;
+    memset(&p, 0, sizeof p);
+    mx_make_map(&p.w, W.codes, W.rows, W.cols, kMxBoxRows);
+    mx_make_scale_map(&p.w_sf, W.scales, W.rows, W.cols, 1);
+    p.src = src; p.src_scales = static_cast<const uint8_t*>(scales); p.src_kind = kind;
+    p.rows = rows; p.n = W.rows; p.k = W.cols;
+    p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
+    cuda_ok(launch_mx_decode(p, s), "matmul_mxfp4 launch");
+}
+
 void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
+    if (mx_decode_form(rows, 1, W.cols)) return few_rows(codes, scales, kMxSrcTiles, rows, W, Y, dtype, status, s);
     MxGemm p;
     memset(&p, 0, sizeof p);
     const int sms = sm_count();
@@ -211,8 +246,8 @@ void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_wei
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
     p.form = mx_form(rows, 1, p.n, sms, 256);
     p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
-    mx_make_map(&p.act, codes, rows, p.k, kMxActRows[p.form]);
-    mx_make_map(&p.w, W.codes, p.n, p.k, kMxWeightRows[p.form]);
+    mx_make_map(&p.act, codes, rows, p.k, kMxBoxRows);
+    mx_make_map(&p.w, W.codes, p.n, p.k, kMxBoxRows);
     if (p.form == kMxPair) {
         mx_make_scale_map(&p.act_sf, scales, rows, p.k, kMxActBands);
         mx_make_scale_map(&p.w_sf, W.scales, p.n, p.k, kMxWeightBands);
@@ -262,6 +297,10 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         if (work_bytes < tmt_moe_linear_mxfp4_work_bytes(rows, W->cols)) throw std::runtime_error("work buffer too small (tmt_moe_linear_mxfp4_work_bytes)");
         check_tensors({X, W->codes, W->scales, Y, work});
         cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (mx_decode_form(rows, 1, W->cols)) {
+            few_rows(X, nullptr, x_dtype == TMT_MOE_F32 ? kMxSrcF32 : kMxSrcBf16, rows, *W, Y, y_dtype, status, s);
+            return 0;
+        }
         uint8_t* codes = static_cast<uint8_t*>(work);
         uint8_t* scales = codes + codes_bytes(rows, W->cols);
         cuda_ok(launch_mx4_quantize(X, x_dtype == TMT_MOE_F32, rows, W->cols, codes, scales, s, true), "quantize_mxfp4 launch");

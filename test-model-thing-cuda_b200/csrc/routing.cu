@@ -367,21 +367,33 @@ __device__ __forceinline__ void scan_finish_dev(const RouteDims& d, const RouteB
         for (int e = threadIdx.x; e < E; e += blockDim.x) cnt_s[e] = b.counts[e];
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 32) {              // prefix sums of the true and the padded counts, 32 experts at a time
+        const int lane = threadIdx.x;
         int tk = 0, ptk = 0;
-        for (int e = 0; e < E; ++e) {
-            const int c = cnt_s[e];
-            b.off[e] = tk; tk += c;
-            poff_s[e] = ptk; b.poff[e] = ptk;
-            ptk += (c + d.pad - 1) / d.pad * d.pad;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane;
+            const int c = e < E ? cnt_s[e] : 0, pc = (c + d.pad - 1) / d.pad * d.pad;
+            int ic = c, ip = pc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int nc = __shfl_up_sync(0xffffffffu, ic, o), np = __shfl_up_sync(0xffffffffu, ip, o);
+                if (lane >= o) { ic += nc; ip += np; }
+            }
+            if (e < E) { b.off[e] = tk + ic - c; poff_s[e] = ptk + ip - pc; b.poff[e] = ptk + ip - pc; }
+            tk += __shfl_sync(0xffffffffu, ic, 31);
+            ptk += __shfl_sync(0xffffffffu, ip, 31);
         }
-        b.off[E] = tk; poff_s[E] = ptk; b.poff[E] = ptk;
-        if (ptk > d.cap) { report(b.status, kErrSlotRange); ptk = 0; }
-        *b.num_m_tiles = ptk / kPad;
-        if (b.use_acc) b.use_acc[E] += 1;
+        if (lane == 0) {
+            b.off[E] = tk; poff_s[E] = ptk; b.poff[E] = ptk;
+            if (ptk > d.cap) { report(b.status, kErrSlotRange); ptk = 0; }
+            *b.num_m_tiles = ptk / kPad;
+        }
     }
-    if (b.use_acc)      // router-balance telemetry: usage accumulated on the device, read when the host asks
-        for (int e = threadIdx.x; e < E; e += blockDim.x) b.use_acc[e] += cnt_s[e];
+    // router-balance telemetry: usage accumulated on the device, read when the host asks (additions nobody waits for)
+    if (b.use_acc) {
+        for (int e = threadIdx.x; e < E; e += blockDim.x) atomicAdd(reinterpret_cast<unsigned long long*>(b.use_acc + e), (unsigned long long)cnt_s[e]);
+        if (threadIdx.x == blockDim.x - 1) atomicAdd(reinterpret_cast<unsigned long long*>(b.use_acc + E), 1ull);
+    }
     __syncthreads();
     const int used = poff_s[E] <= d.cap ? poff_s[E] / kPad : 0;
     for (int i = threadIdx.x; i < d.max_tiles; i += blockDim.x) {
@@ -416,8 +428,10 @@ __global__ void __launch_bounds__(128) router_logits_small_kernel(const RouterAr
     extern __shared__ __align__(16) uint16_t xs[];       // LN: the normalised row
     const int s = threadIdx.x & 7, grp = threadIdx.x >> 3;
     const long t = blockIdx.x;
-    pdl_begin();
+    // The first kernel of a step waits before it lets the next one start: whatever came before the step is then done when any
+    // later kernel of the step begins, and those may read the weights at once.
     pdl_wait();
+    pdl_begin();
     const int nvec = a.D >> 3;
     const unsigned full = 0xffffffffu;
     const uint16_t* xrow = a.X + t * a.D;

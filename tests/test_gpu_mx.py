@@ -129,7 +129,8 @@ def random_blocks(rows, cols, rng, lo=125, hi=130):
 @pytest.mark.parametrize("rows,n,k", [(1, 8, 64), (1, 128, 256), (2, 136, 128), (31, 64, 192), (32, 256, 512), (33, 264, 320), (64, 128, 1024),
                                       (65, 2504, 448), (127, 72, 256), (128, 128, 256), (129, 384, 1344), (257, 512, 576), (500, 1000, 2048),
                                       (1000, 136, 64), (1, 2048, 4096), (20, 4096, 64), (2300, 2056, 320),
-                                      (4096, 1288, 64), (3000, 2504, 448), (5000, 1160, 1344), (2049, 4096, 2048), (9000, 128, 256)])
+                                      (4096, 1288, 64), (3000, 2504, 448), (5000, 1160, 1344), (2049, 4096, 2048), (9000, 128, 256),
+                                      (5, 136, 8192), (32, 264, 5120), (3, 64, 8256), (24, 1000, 1088)])
 def test_matmul_is_exact_where_fp32_is(rows, n, k, dtype):
     rng = np.random.default_rng(rows * 31 + n + k)
     ac, asc, a = random_blocks(rows, k, rng)
@@ -207,7 +208,8 @@ def experts_ref(x, up, down, idx, w):
 @pytest.mark.parametrize("T,D,H,E,K,f32,skew", [(1, 64, 64, 1, 1, False, False), (1, 128, 256, 4, 2, True, False), (64, 256, 512, 16, 2, False, False),
                                                (63, 192, 320, 8, 4, True, True), (300, 128, 64, 3, 2, True, False), (1000, 512, 192, 5, 3, False, False),
                                                (2041, 256, 128, 4, 2, True, True), (700, 64, 128, 64, 8, True, False),
-                                               (6000, 1152, 1344, 5, 3, True, False), (9001, 640, 576, 16, 4, False, True)])
+                                               (6000, 1152, 1344, 5, 3, True, False), (9001, 640, 576, 16, 4, False, True),
+                                               (60, 5120, 64, 4, 2, True, True), (200, 128, 1088, 48, 8, False, False), (2, 256, 192, 32, 2, False, False)])
 @pytest.mark.parametrize("beta", [0.0, 1.0])
 def test_experts_forward(T, D, H, E, K, f32, skew, beta):
     x, wr, up, down = experts_case(T, D, H, E, K, T + D + E, skew)
