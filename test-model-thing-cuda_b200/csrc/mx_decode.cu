@@ -211,7 +211,6 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     const uint32_t codes_w = base, act = codes_w + stages * kCodesW, sf_w = act + nkb * kStageA;      // 1024-byte multiples throughout
     volatile int* abort_flag = &abort_s;
 
-    if (p.early) pdl_begin();
     const CUtensorMap* map = p.w_maps ? p.w_maps + e : &p.w;
     const CUtensorMap* sf_map = p.w_sf_maps ? p.w_sf_maps + e : &p.w_sf;
     auto load_stage = [&](int s, int kb) {
@@ -237,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (p.early) pdl_begin();            // not before: the next kernel could take the tensor memory this one is about to ask for
     }
     __syncwarp();
     pdl_wait();

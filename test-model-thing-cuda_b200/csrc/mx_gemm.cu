@@ -123,7 +123,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     const uint32_t codes_p = base, codes_q = base + S::kStages * S::kCodesP, sf_p = codes_q + S::kStages * S::kCodesQ, sf_q = sf_p + S::kStages * S::kSfP;
     volatile int* abort_flag = &abort_s;
 
-    pdl_begin();
     if (threadIdx.x == 0) {
         abort_s = 0;
         for (int s = 0; s < S::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&empty_bar[s]), 1); }
@@ -134,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(S::kCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_begin();                         // not before: the next kernel could take the tensor memory this one is about to ask for
     }
     pdl_wait();
     load_groups<TA>(p, groups);

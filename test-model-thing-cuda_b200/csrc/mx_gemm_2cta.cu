@@ -20,7 +20,6 @@
 // 200 clocks). An epilogue thread owns a row: it loads 64 columns, hands them back, and works from registers; outputs are staged
 // in shared memory and written by TMA stores.
 // Waits are bounded as in the bf16 kernels; both CTAs always reach the closing cluster barrier before tensor memory is freed.
-#include "launch_pdl.cuh"
 #include "mx_gemm.cuh"
 
 namespace tmt {
@@ -131,7 +130,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
     const uint32_t out_s = sf_w + kStages * kSfW;
     volatile int* abort_flag = &abort_s;
 
-    pdl_begin();
     if (threadIdx.x == 0) {
         abort_s = 0;
         for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 3); mbar_init(smem_u32(&empty_bar[s]), 1); }
@@ -143,7 +141,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
     load_groups<2 * kRows>(p, groups);
     tc_fence_before();
     __syncthreads();
@@ -347,7 +344,11 @@ template <int EPI>
 cudaError_t launch_t(const MxGemm& p, int grid, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(mx_gemm_2cta_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(mx_gemm_2cta_kernel<EPI>, dim3(grid), dim3(kThreads), kSmem, stream, p);
+    // An ordinary launch: no part in the programmatic chains of the short kernels. With the early start on both sides (the quantiser
+    // of the next call resident and waiting while this kernel's clusters ran), a queue of twenty dense layers stood still after eight,
+    // with no wait inside this kernel running out; a kernel of this length has nothing to gain from an early start anyway.
+    mx_gemm_2cta_kernel<EPI><<<grid, kThreads, kSmem, stream>>>(p);
+    return cudaGetLastError();
 }
 
 }  // namespace

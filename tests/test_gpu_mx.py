@@ -307,3 +307,60 @@ def test_ln_backward_act8_against_float64(rows, dim, fmt):
     again = [torch.empty_like(t) for t in (dX, dg, db)]
     M.ln_backward_act8(codes, scales, dY, gamma, mean, rstd, again[0][:rows], again[1], again[2], poisoned(need), FMT8[fmt])
     assert torch.equal(again[0][:rows], dX[:rows]) and torch.equal(again[1], dg) and torch.equal(again[2], db)
+
+
+def test_many_calls_queued_on_one_stream():
+    """Dense layers of every form queued without a wait between them, 20 deep and more: the same bits as one at a time."""
+    torch.manual_seed(5)
+    cases = []
+    for rows, n, k in [(16384, 1024, 1024), (777, 512, 1024), (1, 2048, 1024), (8192, 1024, 512)]:
+        wc, wsc = poisoned(n * k // 2), poisoned(M.mxfp4_scale_bytes(n, k))
+        M.quantize_mxfp4(torch.randn(n, k, device="cuda"), wc, wsc)
+        X = torch.randn(rows, k, device="cuda").bfloat16()
+        Y = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+        cases.append((X, M.Mxfp4Weights([(wc, wsc, n, k)]), Y, poisoned(M.linear_mxfp4_work_bytes(rows, k))))
+    want = []
+    for X, W, Y, work in cases:
+        M.linear_mxfp4(X, W, Y, work)
+        torch.cuda.synchronize()
+        want.append(Y.clone())
+        Y.fill_(float("nan"))
+    for depth in (3, 20, 100):
+        for X, W, Y, work in cases:
+            for _ in range(depth):
+                M.linear_mxfp4(X, W, Y, work)
+        for _ in range(depth):
+            for X, W, Y, work in cases:
+                M.linear_mxfp4(X, W, Y, work)
+        torch.cuda.synchronize()
+        for (_, _, Y, _), y in zip(cases, want):
+            assert torch.equal(Y, y)
+            Y.fill_(float("nan"))
+
+
+def test_many_experts_passes_queued_on_one_stream():
+    torch.manual_seed(6)
+    T, D, H, E, K = 4096, 256, 512, 4, 2
+    moe = M.MoE(T, D, E, K, hidden=H, training=False)
+    up = M.Mxfp4Weights(quantized([w.numpy() for w in torch.randn(E, H, D) * 0.05]))
+    down = M.Mxfp4Weights(quantized([w.numpy() for w in torch.randn(E, D, H) * 0.05]))
+    Wr = (torch.randn(E, D, device="cuda") * 0.05).bfloat16()
+    X = torch.randn(T, D, device="cuda").bfloat16()
+    calls = [(X, torch.empty_like(X)), (X[:300], torch.empty_like(X[:300])), (X[:7], torch.empty_like(X[:7]))]      # many, some, few rows
+    want = []
+    for x, y in calls:
+        moe.forward_mxfp4(x, Wr, up, down, y, 0.0, tokens=len(x))
+        torch.cuda.synchronize()
+        want.append(y.clone())
+        y.zero_()
+    for depth in (3, 20, 100):
+        for x, y in calls:
+            for _ in range(depth):
+                moe.forward_mxfp4(x, Wr, up, down, y, 0.0, tokens=len(x))
+        for _ in range(depth):
+            for x, y in calls:
+                moe.forward_mxfp4(x, Wr, up, down, y, 0.0, tokens=len(x))
+        assert moe.device_status() == 0
+        for (_, y), w in zip(calls, want):
+            assert torch.equal(y, w)
+            y.zero_()
