@@ -2,7 +2,8 @@
 //
 // A warp takes 256 neighbouring elements of a row, 8 per lane, so that a block of 32 is 4 lanes: one 16-byte load per lane
 // (two for fp32), the block's largest magnitude by two shuffles, one store of 4 (e2m1) or 8 bytes (e4m3, e5m2) per lane. Every
-// byte moves once; bound by HBM. Several such chunks are in flight per warp where there are enough of them (U).
+// byte moves once; bound by HBM. In 4 bits a warp takes the same 256 columns of the rows r, r + 32, r + 64 and r + 96 of a band of 128,
+// whose scale words are neighbours in the scale tile (single words, one row a warp, took 150 us instead of 114 at 131072 x 2048). Several such chunks are in flight per warp where there are enough of them (U).
 // `early`: lets the next kernel of the stream be scheduled at once (launch_pdl.cuh). Only where that kernel is known to wait
 // before it reads what this one writes: the product of a dense layer, which starts on its weights without waiting.
 #include <cuda_runtime.h>
@@ -66,17 +67,19 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __res
     Vec8<F32> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const unsigned c = c0 + u;
+        const unsigned c = FMT == kE2M1 ? c0 / U : c0 + u;
         row[u] = c / per_row;
         col[u] = (int)(c - row[u] * per_row) * kChunk + lane * 8;
-        ok[u] = c < chunks && col[u] < cols;                  // cols is a multiple of 32: whole blocks
+        if (FMT == kE2M1) row[u] = (row[u] >> 5) * 128 + (row[u] & 31) + u * 32;      // rows r, r + 32, r + 64, r + 96 of a band
+        ok[u] = c < chunks && row[u] < rows && col[u] < cols;                             // cols is a multiple of 32: whole blocks
         at[u] = (size_t)row[u] * cols + col[u];
         v[u] = Vec8<F32>{};
         if (ok[u]) v[u] = load8<F32>(X, at[u]);
     }
+    uint32_t word[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (c0 + u >= chunks) break;                          // whole warps leave together
+        if (FMT != kE2M1 && c0 + u >= chunks) break;          // whole warps leave together
         float f[8];
         uint32_t m = spread8<F32>(v[u], f);
         m = max(m, __shfl_xor_sync(full, m, 1));
@@ -91,9 +94,7 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __res
             if (ok[u]) *reinterpret_cast<uint32_t*>(codes + at[u] / 2) = q;
             uint32_t w = ok[u] ? sb << (8 * ((lane >> 2) & 3)) : 0u;      // the word of 4 blocks; blocks past the last column are 0
             w |= __shfl_xor_sync(full, w, 4);
-            w |= __shfl_xor_sync(full, w, 8);
-            if ((lane & 15) == 0 && ok[u])
-                *reinterpret_cast<uint32_t*>(scales + scale_word(row[u], col[u] >> 7, scale_tiles_k(cols))) = w;
+            word[u] = w | __shfl_xor_sync(full, w, 8);
         } else {
             uint32_t lo = pack_f8x4<FMT>(f[0], f[1], f[2], f[3]), hi = pack_f8x4<FMT>(f[4], f[5], f[6], f[7]);
             if (sb == 255u) { lo = 0; hi = 0; }
@@ -102,6 +103,12 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __res
                 if ((lane & 3) == 0) scales[at[u] >> 5] = (uint8_t)sb;
             }
         }
+    }
+    if constexpr (FMT == kE2M1) {
+        // the four words of rows r .. r + 96 are neighbours in the scale tile: one 16-byte store (rows past the last: 0, inside the tile)
+        static_assert(FMT != kE2M1 || U == 4, "one row of each quarter of a band");
+        if ((lane & 15) == 0 && ok[0])
+            stg16(scales + scale_word(row[0], col[0] >> 7, scale_tiles_k(cols)), make_uint4(word[0], word[1], word[2], word[3]));
     }
 }
 
@@ -158,10 +165,18 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t* 
 
 struct Grid { unsigned chunks, per_row; int u; dim3 grid; };
 
-Grid plan(long long rows, int cols) {
+// bands: chunks are counted over 32 rows of every band of 128 (4-bit quantiser: a warp takes four rows of a band at once)
+Grid plan(long long rows, int cols, bool bands = false) {
     Grid g;
     g.per_row = (unsigned)((cols + kChunk - 1) / kChunk);
     if (rows > 0x7fffffffLL / g.per_row) throw std::runtime_error("rows * cols exceeds the supported range");
+    if (bands) {
+        const long long r = rows / 128 * 32 + (rows % 128 < 32 ? rows % 128 : 32);
+        g.chunks = (unsigned)(r * g.per_row);
+        g.u = 4;
+        g.grid = dim3((g.chunks + kWarps - 1) / kWarps);
+        return g;
+    }
     g.chunks = (unsigned)(rows * g.per_row);
     // few chunks: one per warp, spread over the SMs; many: four loads in flight per lane
     g.u = g.chunks < 16384u ? 1 : 4;
@@ -171,10 +186,13 @@ Grid plan(long long rows, int cols) {
 
 template <int FMT>
 cudaError_t quantize_t(const void* X, bool f32, long long rows, int cols, uint8_t* codes, uint8_t* scales, cudaStream_t s, bool early = false) {
-    const Grid g = plan(rows, cols);
+    const Grid g = plan(rows, cols, FMT == kE2M1);
     auto go = [&](auto kernel) { return launch_pdl(kernel, g.grid, dim3(kThreads), 0, s, X, (unsigned)rows, cols, g.chunks, g.per_row, codes, scales, early); };
-    if (f32) return g.u == 1 ? go(mx_quantize_kernel<FMT, true, 1>) : go(mx_quantize_kernel<FMT, true, 4>);
-    return g.u == 1 ? go(mx_quantize_kernel<FMT, false, 1>) : go(mx_quantize_kernel<FMT, false, 4>);
+    if constexpr (FMT == kE2M1) return f32 ? go(mx_quantize_kernel<FMT, true, 4>) : go(mx_quantize_kernel<FMT, false, 4>);
+    else {
+        if (f32) return g.u == 1 ? go(mx_quantize_kernel<FMT, true, 1>) : go(mx_quantize_kernel<FMT, true, 4>);
+        return g.u == 1 ? go(mx_quantize_kernel<FMT, false, 1>) : go(mx_quantize_kernel<FMT, false, 4>);
+    }
 }
 
 template <int FMT>

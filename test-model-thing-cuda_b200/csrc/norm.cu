@@ -68,14 +68,20 @@ __global__ void __launch_bounds__(kFwdWarps * 32) ln_fwd_kernel(const uint16_t* 
             fetch(r, raw);
         }
         float sum = 0.0f, sq = 0.0f;
+        uint32_t amax[FMT != 0 ? NV : 1];                // largest magnitude of a lane's vector (bf16 magnitudes order like their bits)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int v = lane + i * 32;
+            if (FMT != 0) amax[FMT != 0 ? i : 0] = 0;
             if (v < nvec) {
                 float f[8];
                 unpack8(raw[i], f);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) { sum = __fadd_rn(sum, f[q]); sq = __fmaf_rn(f[q], f[q], sq); }
+                if constexpr (FMT != 0) {
+                    const uint32_t m = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+                    amax[i] = max(m >> 16, m & 0xffffu) << 16;
+                }
             }
         }
         sum = butterfly(sum);
@@ -89,37 +95,37 @@ __global__ void __launch_bounds__(kFwdWarps * 32) ln_fwd_kernel(const uint16_t* 
         for (int i = 0; i < NV; ++i) {
             const int v = lane + i * 32;
             if (v < nvec) {
-                float f[8], o[8];
+                float f[8];
                 unpack8(raw[i], f);
                 const float4 g0 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8)), g1 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8) + 1);
                 const float4 b0 = __ldg(reinterpret_cast<const float4*>(beta + v * 8)), b1 = __ldg(reinterpret_cast<const float4*>(beta + v * 8) + 1);
-                const float gg[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-                const float bb[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                // packed pairs: each half is the scalar operation, rounded to nearest, so the bits are those stated in the header
+                const float2 gg[4] = {make_float2(g0.x, g0.y), make_float2(g0.z, g0.w), make_float2(g1.x, g1.y), make_float2(g1.z, g1.w)};
+                const float2 bb[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y), make_float2(b1.z, b1.w)};
+                const float2 nm = make_float2(-m, -m), r2 = make_float2(rs, rs);
+                uint32_t o[4];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) o[q] = __fmaf_rn(__fmul_rn(__fsub_rn(f[q], m), rs), gg[q], bb[q]);
-                stg16(y + v * 8, make_uint4(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]), pack_bf2(o[4], o[5]), pack_bf2(o[6], o[7])));
-            }
-        }
-        if constexpr (FMT != 0) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int v = lane + i * 32;
-                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                uint32_t m = 0;                       // magnitudes of bf16 order like their bits
-                if (v < nvec) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) m = __vmaxu2(m, w[q] & 0x7fff7fffu);
+                for (int q = 0; q < 4; ++q) {
+                    const float2 t = __ffma2_rn(__fmul2_rn(__fadd2_rn(make_float2(f[2 * q], f[2 * q + 1]), nm), r2), gg[q], bb[q]);
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[q]) : "f"(t.y), "f"(t.x));
                 }
-                m = max(m >> 16, m & 0xffffu) << 16;
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                if (v < nvec) {                       // dim is a multiple of 32: the four lanes of a block agree
-                    const uint32_t sb = mx::scale_byte<FMT>(m);
+                stg16(y + v * 8, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+            if constexpr (FMT != 0) {                    // dim is a multiple of 32: the four lanes of a block agree on v < nvec
+                uint32_t a = amax[i];
+                a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                if (v < nvec) {
+                    const uint32_t sb = mx::scale_byte<FMT>(a);
                     const float inv = mx::inv_scale(sb);
                     float f[8];
                     unpack8(raw[i], f);
-                    uint32_t lo = mx::pack_f8x4<FMT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-                    uint32_t hi = mx::pack_f8x4<FMT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                    const float2 i2 = make_float2(inv, inv);
+                    float2 p[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) p[q] = __fmul2_rn(make_float2(f[2 * q], f[2 * q + 1]), i2);
+                    uint32_t lo = mx::pack_f8x4<FMT>(p[0].x, p[0].y, p[1].x, p[1].y);
+                    uint32_t hi = mx::pack_f8x4<FMT>(p[2].x, p[2].y, p[3].x, p[3].y);
                     if (sb == 255u) { lo = 0; hi = 0; }
                     *reinterpret_cast<uint2*>(codes + r * D + v * 8) = make_uint2(lo, hi);
                     if ((lane & 3) == 0) scales[r * (D >> 5) + (v >> 2)] = (uint8_t)sb;

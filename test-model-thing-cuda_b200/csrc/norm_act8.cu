@@ -4,11 +4,16 @@
 //   dx = rstd * (g - a - xh * b),   dGamma[d] = sum over rows of dy * xh,   dBeta[d] = sum over rows of dy
 //
 // x is never written out: an element enters as its code, and xh = fma(code, scale * rstd, -mean * rstd).
-// A team walks a contiguous range of rows; a thread owns 8 neighbouring columns (16 bytes of dY, 8 bytes of codes) of every row,
-// so gamma and the column sums stay in its registers. A team is a block of ceil(dim / 256) warps, or for dim < 256 the
-// smallest power of two of lanes that covers a row. RI rows are reduced together: their 2 * RI row sums go through one
-// transposing butterfly (each step halves the values a lane carries: 9 shuffles for 8 sums instead of 40) and one barrier,
-// and the next RI rows are already on their way into registers. The products run on the packed fp32 pair instructions.
+// A team walks a contiguous range of rows; a thread owns one vector of 8 columns (16 bytes of dY, 8 bytes of codes) of every row
+// (V = 2 vectors, half a row apart, where dim > 2048), so gamma and the column sums stay in its registers. A team is a block of
+// ceil(dim / 256) warps; for dim < 256 it is the smallest power of two of lanes that covers a row. RI rows are reduced together:
+// their 2 * RI row sums go through one transposing butterfly (each step halves the values a lane carries: 9 shuffles for 8
+// sums instead of 40) and one barrier. Rows travel through a ring of P rows in shared memory filled by cp.async; every thread
+// copies exactly the pieces it will read itself, so the ring needs no barrier, and its depth costs no registers. The products run
+// on the packed fp32 pair instructions.
+// Measured at 131072 x 2048 (e4m3): 270 us = 5.0 TB/s, 0.77 of the copy rate; bound by issue slots (70 % busy). Two rows a turn and
+// three blocks an SM: 284-315; rows dealt round instead of in ranges: 380; two vectors a thread and four blocks: 375; the
+// row fetched ahead into registers instead of the ring: 343-365.
 // The column sums of the teams are added by a second kernel in a fixed order: results do not depend on timing.
 // Bound: HBM, 5.03 bytes per element (2 + 33/32 read, 2 written).
 #include <algorithm>
@@ -33,7 +38,23 @@ __device__ __forceinline__ uint32_t pack2(float2 v) {
     return r;
 }
 
-struct Raw { uint4 dy; uint2 x; uint32_t sb; float mean, rstd; };
+template <int V> struct Raw { uint32_t sb[V]; float mean, rstd; };      // what of a row does not go through the ring
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
 
 // Sums of N = 4 or 8 values over the 32 lanes of a warp. Afterwards lane l holds the sum of value l / (32 / N).
 template <int N>
@@ -54,72 +75,121 @@ __device__ __forceinline__ float transpose_sum(float (&v)[N], int lane) {
     return s;
 }
 
-// L: lanes of a team (32: the whole block). RI: rows reduced together. MAXT: most threads of a block.
-template <int FMT, int L, int RI, int MAXT>
-__global__ void __launch_bounds__(MAXT) ln_bwd_act8_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+// V: vectors of a thread. L: lanes of a team (32: the whole block). RI: rows reduced together. P: rows of the ring (one commit group each), a multiple of RI.
+// MAXT: most threads of a block, MINB: blocks an SM holds at that size.
+template <int FMT, int V, int L, int RI, int P, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_bwd_act8_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                            const uint16_t* __restrict__ dY, const float* __restrict__ gamma,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                            uint16_t* __restrict__ dX, float* __restrict__ part, int rows, int D,
-                                                           int rows_per_team) {
-    constexpr int NS = 2 * RI;
+                                                           int teams) {
+    static_assert(P % RI == 0, "the ring is refilled RI rows at a time");
+    constexpr int NS = 2 * RI;                               // row sums of a turn
+    extern __shared__ __align__(16) uint8_t ring_raw[];      // [P] x [V] x { 16 bytes of dY, 8 of codes } per thread
     __shared__ float red[2][NS][32];             // [parity][row sums][warp]
-    pdl_begin();
     pdl_wait();
+    pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int team = L == 32 ? (int)blockIdx.x : (int)(blockIdx.x * blockDim.x + threadIdx.x) / L;
-    const int v = L == 32 ? (int)threadIdx.x : lane % L;           // this thread's vector of 8 columns
-    const bool col_ok = v * 8 < D;
-    const float inv_d = 1.0f / (float)D;
-    float2 gam[4], dg[4], db[4];
+    const int c0 = (L == 32 ? (int)threadIdx.x : lane % L) * 8;    // first column of this thread's first vector
+    const int cstep = blockDim.x * 8;                              // from there to the second
+    bool ok[V];
+    float2 gam[V][4], dg[V][4], db[V][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        gam[i] = col_ok ? make_float2(gamma[v * 8 + 2 * i], gamma[v * 8 + 2 * i + 1]) : bc(0.0f);
-        dg[i] = bc(0.0f); db[i] = bc(0.0f);
-    }
-    const long r0 = (long)team * rows_per_team;
-    const long r1 = min(r0 + rows_per_team, (long)rows);
-    auto fetch = [&](long r, Raw& w) {
-        w.dy = make_uint4(0, 0, 0, 0); w.x = make_uint2(0, 0); w.sb = 127; w.mean = 0.0f; w.rstd = 0.0f;
-        if (r < r1) {
-            w.mean = __ldg(mean + r); w.rstd = __ldg(rstd + r);
-            if (col_ok) {
-                w.dy = ldg16_stream(dY + r * D + v * 8);
-                w.x = __ldg(reinterpret_cast<const uint2*>(codes + r * D + v * 8));
-                w.sb = __ldg(scales + r * (D >> 5) + (v >> 2));
-            }
+    for (int k = 0; k < V; ++k) {
+        ok[k] = c0 + k * cstep < D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* p = gamma + c0 + k * cstep + 2 * i;
+            gam[k][i] = ok[k] ? make_float2(p[0], p[1]) : bc(0.0f);
+            dg[k][i] = bc(0.0f); db[k][i] = bc(0.0f);
         }
-    };
-    Raw nxt[RI];
+    }
+    const float inv_d = 1.0f / (float)D;
+    const int rpt = (rows + teams - 1) / teams;      // rows of a team
+    const long first = (long)team * rpt;
+    const int n = (int)max(0L, min((long)rpt, rows - first));
+    const uint32_t vec_bytes = blockDim.x * 24, slot_bytes = V * vec_bytes;
+    const uint32_t ring_dy = (uint32_t)__cvta_generic_to_shared(ring_raw) + threadIdx.x * 16;
+    const uint32_t ring_x = (uint32_t)__cvta_generic_to_shared(ring_raw) + blockDim.x * 16 + threadIdx.x * 8;
+    // running addresses: of the next row to copy, to fetch, to write
+    const uint16_t* p_dy = dY + first * D + c0;
+    const uint8_t* p_x = codes + first * D + c0;
+    const uint8_t* p_sb = scales + first * (D >> 5) + (c0 >> 5);
+    const float* p_mean = mean + first;
+    const float* p_rstd = rstd + first;
+    uint16_t* p_dx = dX + first * D + c0;
+    const int step_sb = D >> 5;
+    int copied = 0, fetched = 0;
+    auto issue = [&](int slot) {                     // one commit group per row, also past the end: the count stays uniform
+        if (copied < n) {
 #pragma unroll
-    for (int j = 0; j < RI; ++j) fetch(r0 + j, nxt[j]);
-    int par = 0;
+            for (int k = 0; k < V; ++k)
+                if (ok[k]) {
+                    copy16(ring_dy + slot * slot_bytes + k * vec_bytes, p_dy + k * cstep);
+                    copy8(ring_x + slot * slot_bytes + k * vec_bytes, p_x + k * cstep);
+                }
+        }
+        copy_commit();
+        ++copied; p_dy += D; p_x += D;
+    };
+    auto fetch = [&](Raw<V>& w) {
+        w.mean = 0.0f; w.rstd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) w.sb[k] = 127;
+        if (fetched < n) {
+            w.mean = __ldg(p_mean); w.rstd = __ldg(p_rstd);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (ok[k]) w.sb[k] = __ldg(p_sb + k * (cstep >> 5));
+        }
+        ++fetched; ++p_mean; ++p_rstd; p_sb += step_sb;
+    };
+#pragma unroll
+    for (int j = 0; j < P; ++j) issue(j);
+    Raw<V> nxt[RI];                                  // one turn ahead
+#pragma unroll
+    for (int j = 0; j < RI; ++j) fetch(nxt[j]);
+    int par = 0, slot0 = 0;
     // every lane of a warp makes the same number of turns (sub-warp teams differ in their last rows alone)
-    for (int turn = 0; turn * RI < rows_per_team; ++turn, par ^= 1) {
-        const long rb = r0 + turn * RI;
-        if (L == 32 && rb >= r1) break;
-        float2 g[RI][4], xh[RI][4];
+    const int n_max = L == 32 ? n : rpt;
+    for (int i0 = 0; i0 < n_max; i0 += RI, par ^= 1) {
+        float2 g[RI][V][4], xh[RI][V][4];
         float rs[RI], s[NS];
+        copy_wait<P - RI>();                         // the RI oldest rows have landed (each thread waits for its own copies)
 #pragma unroll
         for (int j = 0; j < RI; ++j) {
-            const Raw w = nxt[j];
+            const Raw<V> w = nxt[j];
             rs[j] = w.rstd;
-            const float2 sc = bc(scale_value(w.sb) * w.rstd), c = bc(-w.mean * w.rstd);
-            const uint32_t dw[4] = {w.dy.x, w.dy.y, w.dy.z, w.dy.w}, xw[2] = {w.x.x, w.x.y};
+            const float2 c = bc(-w.mean * w.rstd);
             float2 s1 = bc(0.0f), s2 = bc(0.0f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 dy = make_float2(bf_lo(dw[i]), bf_hi(dw[i]));
-                xh[j][i] = __ffma2_rn(unpack_f8x2<FMT>((uint16_t)(xw[i >> 1] >> (16 * (i & 1)))), sc, c);
-                g[j][i] = __fmul2_rn(dy, gam[i]);
-                s1 = __fadd2_rn(s1, g[j][i]);
-                s2 = __ffma2_rn(g[j][i], xh[j][i], s2);
-                dg[i] = __ffma2_rn(dy, xh[j][i], dg[i]);
-                db[i] = __fadd2_rn(db[i], dy);
+            for (int k = 0; k < V; ++k) {
+                uint4 dy4 = make_uint4(0, 0, 0, 0);
+                uint2 x8 = make_uint2(0, 0);
+                if (i0 + j < n && ok[k]) {
+                    const uint32_t at = (slot0 + j) * slot_bytes + k * vec_bytes;
+                    dy4 = lds16(ring_dy + at); x8 = lds8(ring_x + at);
+                }
+                const float2 sc = bc(scale_value(w.sb[k]) * w.rstd);
+                const uint32_t dw[4] = {dy4.x, dy4.y, dy4.z, dy4.w}, xw[2] = {x8.x, x8.y};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 dy = make_float2(bf_lo(dw[i]), bf_hi(dw[i]));
+                    xh[j][k][i] = __ffma2_rn(unpack_f8x2<FMT>((uint16_t)(xw[i >> 1] >> (16 * (i & 1)))), sc, c);
+                    g[j][k][i] = __fmul2_rn(dy, gam[k][i]);
+                    s1 = __fadd2_rn(s1, g[j][k][i]);
+                    s2 = __ffma2_rn(g[j][k][i], xh[j][k][i], s2);
+                    dg[k][i] = __ffma2_rn(dy, xh[j][k][i], dg[k][i]);
+                    db[k][i] = __fadd2_rn(db[k][i], dy);
+                }
             }
             s[2 * j] = s1.x + s1.y; s[2 * j + 1] = s2.x + s2.y;
         }
+        // the slots just read are free (this thread was their only reader)
 #pragma unroll
-        for (int j = 0; j < RI; ++j) fetch(rb + RI + j, nxt[j]);
+        for (int j = 0; j < RI; ++j) { issue(slot0 + j); fetch(nxt[j]); }
+        slot0 = slot0 + RI == P ? 0 : slot0 + RI;
         float tot[NS];
         if constexpr (L == 32) {
             float mine = transpose_sum<NS>(s, lane);                   // value lane / (32 / NS)
@@ -144,20 +214,27 @@ __global__ void __launch_bounds__(MAXT) ln_bwd_act8_kernel(const uint8_t* __rest
 #pragma unroll
         for (int j = 0; j < RI; ++j) {
             const float2 r2 = bc(rs[j]), ca = bc(-rs[j] * (tot[2 * j] * inv_d)), cb = bc(-rs[j] * (tot[2 * j + 1] * inv_d));
-            uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = pack2(__ffma2_rn(xh[j][i], cb, __ffma2_rn(g[j][i], r2, ca)));
-            if (rb + j < r1 && col_ok) stg16(dX + (rb + j) * D + v * 8, make_uint4(o[0], o[1], o[2], o[3]));
+            for (int k = 0; k < V; ++k) {
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = pack2(__ffma2_rn(xh[j][k][i], cb, __ffma2_rn(g[j][k][i], r2, ca)));
+                if (i0 + j < n && ok[k]) stg16(p_dx + k * cstep, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+            p_dx += D;
         }
     }
-    if (col_ok) {
-        float* p = part + (size_t)team * 2 * D + v * 8;
+    copy_wait<0>();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<float2*>(p + 2 * i) = dg[i];
-            *reinterpret_cast<float2*>(p + D + 2 * i) = db[i];
+    for (int k = 0; k < V; ++k)
+        if (ok[k]) {
+            float* p = part + (size_t)team * 2 * D + c0 + k * cstep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                *reinterpret_cast<float2*>(p + 2 * i) = dg[k][i];
+                *reinterpret_cast<float2*>(p + D + 2 * i) = db[k][i];
+            }
         }
-    }
 }
 
 // Column i of [dGamma | dBeta]: 32 partial sums over the teams (teams y, y + 32, ...), then those in a tree.
@@ -179,44 +256,45 @@ __global__ void __launch_bounds__(1024) ln_bwd_act8_reduce_kernel(const float* _
     if (x == 0) { if (c < D) dGamma[c] = s; else dBeta[c - D] = s; }
 }
 
-struct Plan { int lanes, threads, blocks, teams, rows_per_team; };
+struct Plan { int lanes, threads, blocks, teams; };
 
 // From the shape alone (148 SMs): the scratch size and the order of the sums do not depend on where the call runs.
 Plan plan(int rows, int dim) {
     constexpr int kSms = 148, kMinRows = 8;
     Plan p;
-    const int vec = dim / 8;
+    const int threads = (dim / (dim <= 2048 ? 8 : 16) + 31) / 32 * 32;
     p.lanes = 32;
-    while (p.lanes / 2 >= vec) p.lanes /= 2;
-    const int warps = (vec + 31) / 32;
-    p.threads = p.lanes < 32 ? 128 : warps * 32;
+    while (dim <= 256 && p.lanes / 2 >= dim / 8) p.lanes /= 2;
+    p.threads = p.lanes < 32 ? 128 : threads;
     const int per_block = p.lanes < 32 ? p.threads / p.lanes : 1;
-    const int resident = std::max(1, std::min(24, 16 / warps)) * kSms * (p.lanes < 32 ? 4 : 1);
+    const int resident = std::max(1, std::min(24, 512 / p.threads)) * kSms;      // 16 warps an SM hold 128 registers each
     const int want = (rows + kMinRows * per_block - 1) / (kMinRows * per_block);
     p.blocks = std::max(1, std::min(want, resident));
     p.teams = p.blocks * per_block;
-    p.rows_per_team = (rows + p.teams - 1) / p.teams;
     return p;
 }
 
-template <int FMT, int L, int RI, int MAXT>
+template <int FMT, int V, int L, int RI, int P, int MAXT, int MINB>
 cudaError_t launch_t(const Plan& p, cudaStream_t s, const uint8_t* codes, const uint8_t* scales, const uint16_t* dY, const float* gamma,
                      const float* mean, const float* rstd, uint16_t* dX, float* part, int rows, int dim) {
-    return launch_pdl(ln_bwd_act8_kernel<FMT, L, RI, MAXT>, dim3(p.blocks), dim3(p.threads), 0, s, codes, scales, dY, gamma, mean, rstd, dX, part,
-                      rows, dim, p.rows_per_team);
+    auto kernel = ln_bwd_act8_kernel<FMT, V, L, RI, P, MAXT, MINB>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P * MAXT * 24 * V);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3(p.blocks), dim3(p.threads), (size_t)P * p.threads * 24 * V, s, codes, scales, dY, gamma, mean, rstd, dX, part,
+                      rows, dim, p.teams);
 }
 
 template <int FMT, class... A>
-cudaError_t launch_f(const Plan& p, A... a) {
+cudaError_t launch_f(const Plan& p, int dim, A... a) {
     switch (p.lanes) {
-        case 4: return launch_t<FMT, 4, 4, 128>(p, a...);
-        case 8: return launch_t<FMT, 8, 4, 128>(p, a...);
-        case 16: return launch_t<FMT, 16, 4, 128>(p, a...);
+        case 4: return launch_t<FMT, 1, 4, 4, 8, 128, 4>(p, a...);
+        case 8: return launch_t<FMT, 1, 8, 4, 8, 128, 4>(p, a...);
+        case 16: return launch_t<FMT, 1, 16, 4, 8, 128, 4>(p, a...);
         default: break;
     }
-    if (p.threads <= 256) return launch_t<FMT, 32, 4, 256>(p, a...);
-    if (p.threads <= 512) return launch_t<FMT, 32, 4, 512>(p, a...);
-    return launch_t<FMT, 32, 2, 1024>(p, a...);
+    if (dim <= 256) return launch_t<FMT, 1, 32, 4, 8, 32, 16>(p, a...);
+    if (dim <= 2048) return launch_t<FMT, 1, 32, 4, 8, 256, 2>(p, a...);
+    return launch_t<FMT, 2, 32, 2, 4, 512, 1>(p, a...);
 }
 
 }  // namespace
@@ -246,8 +324,8 @@ int tmt_ln_backward_act8(const void* codes, const void* scales, int format, cons
         const uint16_t* dy = static_cast<const uint16_t*>(dY);
         uint16_t* dx = static_cast<uint16_t*>(dX);
         float* part = static_cast<float*>(scratch);
-        cuda_ok(format == kE4M3 ? launch_f<kE4M3>(p, s, c, sc, dy, gamma, mean, rstd, dx, part, rows, dim)
-                                : launch_f<kE5M2>(p, s, c, sc, dy, gamma, mean, rstd, dx, part, rows, dim), "ln_backward_act8 launch");
+        cuda_ok(format == kE4M3 ? launch_f<kE4M3>(p, dim, s, c, sc, dy, gamma, mean, rstd, dx, part, rows, dim)
+                                : launch_f<kE5M2>(p, dim, s, c, sc, dy, gamma, mean, rstd, dx, part, rows, dim), "ln_backward_act8 launch");
         cuda_ok(launch_pdl(ln_bwd_act8_reduce_kernel, dim3(2 * dim / 32), dim3(1024), 0, s, part, p.teams, dim, dGamma, dBeta), "ln_backward_act8 launch");
     })
 }
