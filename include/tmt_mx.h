@@ -17,9 +17,16 @@
  *
  * Conventions as in tmt_moe.h and tmt_norm.h: 0 / -1, message from tmt_moe_last_error(), device pointers, 16-byte aligned
  * (what cudaMalloc returns is), nothing allocates, nothing synchronises, nothing calls exit(). Work is queued on `stream`
- * of the current device; a tensor that lies on another device, or in host memory that the device cannot read, is refused.
- * Calls may run side by side on several streams (they share no state), and may be captured into a graph. rows = 0 is
- * allowed where no handle is involved and does nothing. */
+ * of the current device; a tensor that lies on another device or in host memory is refused. Outputs and workspaces overlap
+ * neither each other nor an input.
+ * Calls without a handle may run side by side on several streams (they share no state), and may be captured into a graph.
+ * rows = 0 is allowed where no handle is involved and does nothing.
+ *
+ * Kernels of these operators may be scheduled while the one before them on the stream is still running (programmatic launch;
+ * TMT_MOE_PDL=0 in the environment switches it off). They wait for it before they touch what it may write, with one exception:
+ * products of few rows ask for their WEIGHTS at once. Weights written by tmt_moe_quantize_mxfp4, by copies, or by any kernel
+ * that does not itself let its successor start early (no ordinary kernel does) are safe; a kernel of the caller's own that
+ * calls griddepcontrol.launch_dependents before it has written a weight is not. */
 #ifndef TMT_MX_H
 #define TMT_MX_H
 
@@ -33,7 +40,7 @@ extern "C" {
 #endif
 
 /* Formats of the 8-bit checkpoints. */
-enum { TMT_ACT8_OFF = 0, TMT_ACT8_E4M3 = 1, TMT_ACT8_E5M2 = 2 };
+enum { TMT_ACT8_E4M3 = 1, TMT_ACT8_E5M2 = 2 };
 
 /* A 4-bit weight matrix W (rows = outputs, cols = inputs), [out,in] as everywhere in tmt_moe.h. */
 typedef struct tmt_mxfp4_weight {
@@ -69,7 +76,8 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
  * on its way into its experts' groups; P = q4(X) Wup^T, then q4(silu(P)) straight from the fp32 accumulators, then
  * gate * (q4(silu(P)) Wdown^T). Wup / Wdown: HOST arrays of E descriptors whose device memory must stay valid while the
  * handle uses them. The first call on a handle allocates its buffers, and a call with other pointers than the last one
- * uploads a table: both outside any stream capture. */
+ * uploads a table and waits for it: both are refused while the handle's stream is being captured. Other calls may be recorded;
+ * a graph keeps the weights' addresses it was recorded with, whatever later calls are given. */
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
                           const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
 

@@ -38,6 +38,7 @@ struct MxState {
     CUtensorMap* tables = nullptr;                 // per-expert weight maps (mx_moe.cu)
     const uint8_t** scale_tab = nullptr;           // [2][E]
     std::vector<const void*> key;                  // the pointers the tables were built from
+    bool recorded = false;                         // a graph was recorded with these tables
 };
 }  // namespace tmt
 

@@ -14,8 +14,8 @@ inline void cuda_ok(cudaError_t e, const char* what) {
     if (e != cudaSuccess) throw std::runtime_error(std::string(what) + " failed: " + cudaGetErrorString(e));
 }
 
-// Every tensor is 16-byte aligned and lies where the current device reaches it: in its own memory, in managed memory or in
-// pinned host memory. A pointer of another device would fault there, so it is refused here.
+// Every tensor is 16-byte aligned and lies in the current device's memory or in managed memory. A pointer of another device or
+// of the host would fault there, so it is refused here.
 inline void check_tensors(std::initializer_list<const void*> ptrs, uintptr_t align = 16) {
     int dev = 0;
     cuda_ok(cudaGetDevice(&dev), "cudaGetDevice");
@@ -24,7 +24,7 @@ inline void check_tensors(std::initializer_list<const void*> ptrs, uintptr_t ali
         if (reinterpret_cast<uintptr_t>(p) & (align - 1)) throw std::runtime_error("a tensor must start on a " + std::to_string(align) + "-byte boundary");
         cudaPointerAttributes a{};
         cuda_ok(cudaPointerGetAttributes(&a, p), "cudaPointerGetAttributes");
-        if (a.type == cudaMemoryTypeUnregistered) throw std::runtime_error("a tensor lies in host memory that the device cannot read");
+        if (a.type == cudaMemoryTypeUnregistered || a.type == cudaMemoryTypeHost) throw std::runtime_error("a tensor lies in host memory");
         if (a.type == cudaMemoryTypeDevice && a.device != dev)
             throw std::runtime_error("a tensor lies on device " + std::to_string(a.device) + ", the current device is " + std::to_string(dev));
     }

@@ -103,9 +103,14 @@ T* alloc(tmt_moe* h, size_t n) {
     return static_cast<T*>(p);
 }
 
+void new_tables(tmt_moe* h) {
+    h->mx.tables = alloc<CUtensorMap>(h, kTables * (size_t)h->d.experts);
+    h->mx.scale_tab = alloc<const uint8_t*>(h, 2 * (size_t)h->d.experts);
+    h->mx.recorded = false;
+}
+
 void make_buffers(tmt_moe* h) {
     MxState& m = h->mx;
-    if (m.tables) return;
     const int D = h->d.dim, H = h->d.hidden, E = h->d.experts;
     const long cap = h->dims.cap;
     m.x_codes = alloc<uint8_t>(h, (size_t)cap * D / 2);
@@ -120,17 +125,32 @@ void make_buffers(tmt_moe* h) {
     // the padding rows' scale bytes are read with the others (their products are never used): give them a value
     cuda_ok(cudaMemsetAsync(m.x_scales, 0, scale_bytes(cap, D), h->stream), "cudaMemsetAsync");
     cuda_ok(cudaMemsetAsync(m.h_scales, 0, scale_bytes(cap, H), h->stream), "cudaMemsetAsync");
-    m.tables = alloc<CUtensorMap>(h, kTables * (size_t)E);
-    m.scale_tab = alloc<const uint8_t*>(h, 2 * (size_t)E);
+    new_tables(h);
 }
 
-// Per-expert maps and scale pointers, uploaded when the caller's pointers changed.
+bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    cuda_ok(cudaStreamIsCapturing(s, &st), "cudaStreamIsCapturing");
+    return st != cudaStreamCaptureStatusNone;
+}
+
+// Per-expert maps and scale pointers of the weights handed in, uploaded when they are not those of the call before. (They are
+// addresses and shapes only; what the weights hold is read at every call.) A recorded graph goes on reading the tables it was
+// recorded with: those are never written again, the next list of weights gets tables of its own.
 void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown) {
     const int E = h->d.experts;
     MxState& m = h->mx;
     std::vector<const void*> key(4 * (size_t)E);
     for (int e = 0; e < E; ++e) { key[e] = Wup[e].scales; key[E + e] = Wdown[e].scales; key[2 * E + e] = Wup[e].codes; key[3 * E + e] = Wdown[e].codes; }
-    if (key == m.key) return;
+    const bool recording = capturing(h->stream);
+    if (m.tables && key == m.key) {
+        m.recorded |= recording;
+        return;
+    }
+    if (recording)
+        throw std::runtime_error("forward_mxfp4: the first call on a handle, and the first one with other weights, cannot be recorded into a graph; make one outside the capture");
+    if (!m.tables) make_buffers(h);
+    if (m.recorded) new_tables(h);
     m.key.clear();                       // stays empty if anything below throws
     for (const void* p : key) check_tensors({p});
     std::vector<CUtensorMap> maps(kTables * (size_t)E);
@@ -158,7 +178,7 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
         if (Wup[e].rows != H || Wup[e].cols != D || Wdown[e].rows != D || Wdown[e].cols != H)
             throw std::runtime_error("MXFP4 weight shape does not match the handle");
     cuda_ok(cudaSetDevice(h->d.device), "cudaSetDevice");
-    make_buffers(h);
+    check_tensors({X, Wr, Y});
     refresh_tables(h, Wup, Wdown);
     MxState& m = h->mx;
     h->dims.T = tokens;
@@ -278,6 +298,7 @@ int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, co
         if (rows < 0) throw std::runtime_error("rows must not be negative");
         if (rows == 0) return 0;
         check_tensors({A_codes, A_scales, W->codes, W->scales, Y});
+        if (status) check_tensors({status}, 4);
         matmul(A_codes, A_scales, rows, *W, Y, dtype, status, static_cast<cudaStream_t>(stream));
     })
 }
@@ -296,6 +317,7 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         if (rows == 0) return 0;
         if (work_bytes < tmt_moe_linear_mxfp4_work_bytes(rows, W->cols)) throw std::runtime_error("work buffer too small (tmt_moe_linear_mxfp4_work_bytes)");
         check_tensors({X, W->codes, W->scales, Y, work});
+        if (status) check_tensors({status}, 4);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (mx_decode_form(rows, 1, W->cols)) {
             few_rows(X, nullptr, x_dtype == TMT_MOE_F32 ? kMxSrcF32 : kMxSrcBf16, rows, *W, Y, y_dtype, status, s);

@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libtmt_moe_b200.so")
 BF16, F32 = 0, 1
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05_2CTA, GEMM_TCGEN05 = 0, 1, 2, 3
 EP_PEER, EP_NCCL, EP_DMA = 0, 1, 2
-ACT8_OFF, ACT8_E4M3, ACT8_E5M2 = 0, 1, 2
+ACT8_E4M3, ACT8_E5M2 = 1, 2
 
 EXPORTS = (
     "tmt_moe_create", "tmt_moe_destroy", "tmt_moe_last_error", "tmt_moe_set_router_bias",
@@ -257,13 +257,13 @@ class MoE:
         down = Wdown if isinstance(Wdown, Mxfp4Weights) else Mxfp4Weights(Wdown)
         if up.n != self.experts or down.n != self.experts:
             raise MoeError("forward_mxfp4 needs one weight per expert (%d), got %d and %d" % (self.experts, up.n, down.n))
-        for name, a in (("X", X), ("Y", Y)):
-            _dense(a, name, ("torch.bfloat16", "torch.int16"))
-            if a.shape[-1] != self.dim or a.numel() < t * self.dim:
-                raise MoeError("%s has too few rows or another width than the handle" % name)
-        _dense(Wrouter, "Wrouter", ("torch.float32",) if self.desc.router_dtype == F32 else ("torch.bfloat16", "torch.int16"))
+        _dense(X, "X", _BF, t * self.dim), _dense(Y, "Y", _BF, t * self.dim)
+        if X.shape[-1] != self.dim or Y.shape[-1] != self.dim:
+            raise MoeError("X and Y must have the handle's width, %d" % self.dim)
+        _dense(Wrouter, "Wrouter", _FP if self.desc.router_dtype == F32 else _BF, self.experts * self.dim)
         self._mx_keep = (up, down)          # the handle keeps a table of their device addresses
-        _check(self.lib.tmt_moe_forward_mxfp4(self.h, X.data_ptr(), Wrouter.data_ptr(), up.arr, down.arr, Y.data_ptr(), beta, t), self.lib)
+        if self.lib.tmt_moe_forward_mxfp4(self.h, X.data_ptr(), Wrouter.data_ptr(), up.arr, down.arr, Y.data_ptr(), beta, t):
+            _check(-1, self.lib)
 
     def nvfp4_weights_changed(self):
         """Call after re-quantising into the same buffers: derived copies are rebuilt at the next forward_nvfp4."""
@@ -528,30 +528,41 @@ def _declare_mx(lib):
         fn.restype, fn.argtypes = res, args
 
 
-_DTYPE = {"torch.bfloat16": BF16, "torch.int16": BF16, "torch.float32": F32}
-_BYTES = ("torch.uint8", "torch.float8_e4m3fn", "torch.float8_e5m2", "torch.float8_e8m0fnu")
+_BYTE = 2                   # beside BF16 and F32: a type of one byte
+_NAMES = {"torch.bfloat16": BF16, "torch.int16": BF16, "torch.float32": F32, "torch.uint8": _BYTE, "torch.float8_e4m3fn": _BYTE,
+          "torch.float8_e5m2": _BYTE, "torch.float8_e8m0fnu": _BYTE}       # int16: raw bf16 patterns, as elsewhere in this package
+_WORDS = {BF16: "bfloat16 (or int16)", F32: "float32", _BYTE: "a type of one byte"}
+_KIND = {}                  # the same by dtype object, filled as they are met
 
 
-def _dense(t, name, dtypes):
-    if not t.is_contiguous():
-        raise MoeError("%s must be contiguous" % name)
-    d = str(t.dtype)
-    if d not in dtypes:
-        raise MoeError("%s has type %s, expected %s" % (name, d, " or ".join(dtypes)))
-    return d
+def _kind(t):
+    k = _KIND.get(t.dtype)
+    if k is None:
+        k = _KIND[t.dtype] = _NAMES.get(str(t.dtype), -1)
+    return k
 
 
-def _values(t, name):
-    """TMT_MOE_BF16 / TMT_MOE_F32 of a dense matrix of values (int16: raw bf16 patterns, as elsewhere in this package)."""
+def _dense(t, name, kinds, need):
+    """Refuses a tensor that is not contiguous, of another type, or shorter than `need` elements; returns its kind."""
+    k = _KIND.get(t.dtype)
+    if k is None:
+        k = _kind(t)
+    if k not in kinds or not t.is_contiguous() or t.numel() < need:
+        if k not in kinds:
+            raise MoeError("%s has type %s, expected %s" % (name, t.dtype, " or ".join(_WORDS[x] for x in kinds)))
+        if not t.is_contiguous():
+            raise MoeError("%s must be contiguous" % name)
+        raise MoeError("%s has %d elements, %d are needed" % (name, t.numel(), need))
+    return k
+
+
+_VALUES, _BF, _FP, _BY = (BF16, F32), (BF16,), (F32,), (_BYTE,)
+
+
+def _matrix(t, name):
     if t.dim() != 2:
         raise MoeError("%s must have two dimensions" % name)
-    return _DTYPE[_dense(t, name, tuple(_DTYPE))]
-
-
-def _bytes(t, name, need):
-    _dense(t, name, _BYTES)
-    if t.numel() < need:
-        raise MoeError("%s holds %d bytes, %d are needed" % (name, t.numel(), need))
+    return t.shape
 
 
 class Mxfp4Weights:
@@ -563,9 +574,10 @@ class Mxfp4Weights:
         self.n = len(entries)
         self.arr = (_Mxfp4WeightDesc * self.n)()
         for i, (c, s, r, k) in enumerate(entries):
-            _bytes(c, "codes", r * k // 2)
-            _bytes(s, "scales", mxfp4_scale_bytes(r, k))
+            _dense(c, "codes", _BY, r * k // 2)
+            _dense(s, "scales", _BY, mxfp4_scale_bytes(r, k))
             self.arr[i] = _Mxfp4WeightDesc(c.data_ptr(), s.data_ptr(), r, k)
+        self.rows, self.cols = (entries[0][2], entries[0][3]) if entries else (0, 0)
         self._keep = entries
 
 
@@ -575,22 +587,32 @@ def mxfp4_scale_bytes(rows, cols):
 
 def quantize_mxfp4(X, codes, scales, stream=None):
     """X (rows, cols) bf16 or fp32 -> 4-bit blocks; codes: rows * cols / 2 bytes, scales: mxfp4_scale_bytes(rows, cols) bytes."""
-    lib = load()
-    dt = _values(X, "X")
-    rows, cols = X.shape
-    _bytes(codes, "codes", rows * cols // 2)
-    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
-    _check(lib.tmt_moe_quantize_mxfp4(X.data_ptr(), dt, rows, cols, codes.data_ptr(), scales.data_ptr(), stream), lib)
+    lib = _lib or load()
+    rows, cols = _matrix(X, "X")
+    dt = _dense(X, "X", _VALUES, 0)
+    _dense(codes, "codes", _BY, rows * cols // 2)
+    _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
+    if lib.tmt_moe_quantize_mxfp4(X.data_ptr(), dt, rows, cols, codes.data_ptr(), scales.data_ptr(), stream):
+        _check(-1, lib)
 
 
 def dequantize_mxfp4(codes, scales, Y, stream=None):
     """4-bit blocks -> Y (rows, cols) bf16 or fp32."""
-    lib = load()
-    dt = _values(Y, "Y")
-    rows, cols = Y.shape
-    _bytes(codes, "codes", rows * cols // 2)
-    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
-    _check(lib.tmt_moe_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, cols, Y.data_ptr(), dt, stream), lib)
+    lib = _lib or load()
+    rows, cols = _matrix(Y, "Y")
+    dt = _dense(Y, "Y", _VALUES, 0)
+    _dense(codes, "codes", _BY, rows * cols // 2)
+    _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
+    if lib.tmt_moe_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, cols, Y.data_ptr(), dt, stream):
+        _check(-1, lib)
+
+
+def _status(t):
+    if t is None:
+        return None
+    if str(t.dtype) != "torch.int32" or t.numel() < 1:
+        raise MoeError("status must be an int32 tensor of one element")
+    return t.data_ptr()
 
 
 def _one_weight(W):
@@ -600,23 +622,24 @@ def _one_weight(W):
     return W
 
 
-def _out_shape(Y, rows, W):
-    dt = _values(Y, "Y")
-    if tuple(Y.shape) != (rows, W.arr[0].rows):
-        raise MoeError("Y has shape %s, expected %s" % (tuple(Y.shape), (rows, W.arr[0].rows)))
-    return dt
+def _out(Y, rows, W):
+    r, n = _matrix(Y, "Y")
+    if r != rows or n != W.rows:
+        raise MoeError("Y has shape %s, expected %s" % (tuple(Y.shape), (rows, W.rows)))
+    return _dense(Y, "Y", _VALUES, 0)
 
 
 def matmul_mxfp4(codes, scales, W, Y, status=None, stream=None):
     """Y (rows, W rows) = A W^T, both in 4-bit blocks; W: Mxfp4Weights with one entry, or (codes, scales, rows, cols)."""
-    lib = load()
+    lib = _lib or load()
     W = _one_weight(W)
-    rows, k = Y.shape[0], W.arr[0].cols
-    dt = _out_shape(Y, rows, W)
-    _bytes(codes, "codes", rows * k // 2)
-    _bytes(scales, "scales", lib.tmt_moe_mxfp4_scale_bytes(rows, k))
-    _check(lib.tmt_moe_matmul_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, W.arr, Y.data_ptr(), dt,
-                                    None if status is None else status.data_ptr(), stream), lib)
+    rows, k = Y.shape[0], W.cols
+    dt = _out(Y, rows, W)
+    _dense(codes, "codes", _BY, rows * k // 2)
+    _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, k))
+    if lib.tmt_moe_matmul_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, W.arr, Y.data_ptr(), dt,
+                                _status(status), stream):
+        _check(-1, lib)
 
 
 def linear_mxfp4_work_bytes(rows, cols):
@@ -625,61 +648,52 @@ def linear_mxfp4_work_bytes(rows, cols):
 
 def linear_mxfp4(X, W, Y, work, status=None, stream=None):
     """Y = q4(X) W^T: X (rows, cols) bf16 or fp32 is quantised into work (linear_mxfp4_work_bytes(rows, cols) bytes) and multiplied."""
-    lib = load()
+    lib = _lib or load()
     W = _one_weight(W)
-    xt = _values(X, "X")
-    rows, k = X.shape
-    if k != W.arr[0].cols:
-        raise MoeError("X has %d columns, the weight %d" % (k, W.arr[0].cols))
-    yt = _out_shape(Y, rows, W)
-    _dense(work, "work", _BYTES)
-    _check(lib.tmt_moe_linear_mxfp4(X.data_ptr(), xt, rows, W.arr, Y.data_ptr(), yt, work.data_ptr(), work.numel(),
-                                    None if status is None else status.data_ptr(), stream), lib)
+    rows, k = _matrix(X, "X")
+    if k != W.cols:
+        raise MoeError("X has %d columns, the weight %d" % (k, W.cols))
+    xt, yt = _dense(X, "X", _VALUES, 0), _out(Y, rows, W)
+    _dense(work, "work", _BY, 0)
+    if lib.tmt_moe_linear_mxfp4(X.data_ptr(), xt, rows, W.arr, Y.data_ptr(), yt, work.data_ptr(), work.numel(),
+                                _status(status), stream):
+        _check(-1, lib)
 
 
 def act8_save(X, codes, scales, fmt=ACT8_E4M3, stream=None):
     """8-bit checkpoint of X (rows, cols) bf16 or fp32; codes: rows * cols bytes, scales: rows * cols / 32 bytes."""
-    lib = load()
-    dt = _values(X, "X")
-    rows, cols = X.shape
-    _bytes(codes, "codes", rows * cols)
-    _bytes(scales, "scales", rows * cols // 32)
-    _check(lib.tmt_moe_act8_save(X.data_ptr(), dt, rows, cols, fmt, codes.data_ptr(), scales.data_ptr(), stream), lib)
+    lib = _lib or load()
+    rows, cols = _matrix(X, "X")
+    dt = _dense(X, "X", _VALUES, 0)
+    _dense(codes, "codes", _BY, rows * cols)
+    _dense(scales, "scales", _BY, rows * cols // 32)
+    if lib.tmt_moe_act8_save(X.data_ptr(), dt, rows, cols, fmt, codes.data_ptr(), scales.data_ptr(), stream):
+        _check(-1, lib)
 
 
 def act8_restore(codes, scales, Y, fmt=ACT8_E4M3, stream=None):
     """The values of an 8-bit checkpoint -> Y (rows, cols) bf16 or fp32."""
-    lib = load()
-    dt = _values(Y, "Y")
-    rows, cols = Y.shape
-    _bytes(codes, "codes", rows * cols)
-    _bytes(scales, "scales", rows * cols // 32)
-    _check(lib.tmt_moe_act8_restore(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, Y.data_ptr(), dt, stream), lib)
-
-
-def _ln_checkpoint(codes, scales, rows, dim):
-    _bytes(codes, "codes", rows * dim)
-    _bytes(scales, "scales", rows * dim // 32)
-
-
-def _vectors(n, **ts):
-    for name, t in ts.items():
-        _dense(t, name, ("torch.float32",))
-        if t.numel() < n:
-            raise MoeError("%s has %d elements, %d are needed" % (name, t.numel(), n))
+    lib = _lib or load()
+    rows, cols = _matrix(Y, "Y")
+    dt = _dense(Y, "Y", _VALUES, 0)
+    _dense(codes, "codes", _BY, rows * cols)
+    _dense(scales, "scales", _BY, rows * cols // 32)
+    if lib.tmt_moe_act8_restore(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, Y.data_ptr(), dt, stream):
+        _check(-1, lib)
 
 
 def ln_forward_act8(X, gamma, beta, Y, mean, rstd, codes, scales, fmt=ACT8_E4M3, stream=None):
     """ln_forward that also leaves an 8-bit checkpoint of X (include/tmt_norm.h): codes rows * dim bytes, scales rows * dim / 32."""
-    lib = load()
-    if _values(X, "X") != BF16 or _values(Y, "Y") != BF16 or X.shape != Y.shape:
-        raise MoeError("X and Y must be bf16 matrices of the same shape")
-    rows, dim = X.shape
-    _vectors(dim, gamma=gamma, beta=beta)
-    _vectors(rows, mean=mean, rstd=rstd)
-    _ln_checkpoint(codes, scales, rows, dim)
-    _check(lib.tmt_ln_forward_act8(X.data_ptr(), gamma.data_ptr(), beta.data_ptr(), Y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                                   codes.data_ptr(), scales.data_ptr(), fmt, rows, dim, stream), lib)
+    lib = _lib or load()
+    rows, dim = _matrix(X, "X")
+    if X.shape != Y.shape:
+        raise MoeError("X and Y must have the same shape")
+    n = rows * dim
+    _dense(X, "X", _BF, 0), _dense(Y, "Y", _BF, 0), _dense(gamma, "gamma", _FP, dim), _dense(beta, "beta", _FP, dim)
+    _dense(mean, "mean", _FP, rows), _dense(rstd, "rstd", _FP, rows), _dense(codes, "codes", _BY, n), _dense(scales, "scales", _BY, n // 32)
+    if lib.tmt_ln_forward_act8(X.data_ptr(), gamma.data_ptr(), beta.data_ptr(), Y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                               codes.data_ptr(), scales.data_ptr(), fmt, rows, dim, stream):
+        _check(-1, lib)
 
 
 def ln_backward_act8_scratch_bytes(rows, dim):
@@ -688,15 +702,15 @@ def ln_backward_act8_scratch_bytes(rows, dim):
 
 def ln_backward_act8(codes, scales, dY, gamma, mean, rstd, dX, dGamma, dBeta, scratch, fmt=ACT8_E4M3, stream=None):
     """ln_backward from the checkpoint ln_forward_act8 left; scratch: ln_backward_act8_scratch_bytes(rows, dim) bytes."""
-    lib = load()
-    if _values(dY, "dY") != BF16 or _values(dX, "dX") != BF16 or dX.shape != dY.shape:
-        raise MoeError("dY and dX must be bf16 matrices of the same shape")
-    rows, dim = dY.shape
-    _vectors(dim, gamma=gamma, dGamma=dGamma, dBeta=dBeta)
-    _vectors(rows, mean=mean, rstd=rstd)
-    _ln_checkpoint(codes, scales, rows, dim)
-    _dense(scratch, "scratch", _BYTES + ("torch.float32",))
-    if scratch.numel() * scratch.element_size() < lib.tmt_ln_backward_act8_scratch_bytes(rows, dim):
-        raise MoeError("scratch is too small (ln_backward_act8_scratch_bytes)")
-    _check(lib.tmt_ln_backward_act8(codes.data_ptr(), scales.data_ptr(), fmt, dY.data_ptr(), gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                                    dX.data_ptr(), dGamma.data_ptr(), dBeta.data_ptr(), rows, dim, scratch.data_ptr(), stream), lib)
+    lib = _lib or load()
+    rows, dim = _matrix(dY, "dY")
+    if dX.shape != dY.shape:
+        raise MoeError("dX and dY must have the same shape")
+    n = rows * dim
+    _dense(dY, "dY", _BF, 0), _dense(dX, "dX", _BF, 0), _dense(gamma, "gamma", _FP, dim), _dense(mean, "mean", _FP, rows)
+    _dense(rstd, "rstd", _FP, rows), _dense(dGamma, "dGamma", _FP, dim), _dense(dBeta, "dBeta", _FP, dim)
+    _dense(codes, "codes", _BY, n), _dense(scales, "scales", _BY, n // 32)
+    _dense(scratch, "scratch", _BY, lib.tmt_ln_backward_act8_scratch_bytes(rows, dim))
+    if lib.tmt_ln_backward_act8(codes.data_ptr(), scales.data_ptr(), fmt, dY.data_ptr(), gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                dX.data_ptr(), dGamma.data_ptr(), dBeta.data_ptr(), rows, dim, scratch.data_ptr(), stream):
+        _check(-1, lib)
