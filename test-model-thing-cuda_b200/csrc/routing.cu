@@ -85,7 +85,12 @@ __device__ __forceinline__ void route_block_finish(const RouterArgs& a, float* l
         for (int j = 0; j < K; ++j) {
             float bv = -INFINITY; int bi = 0x7fffffff;
             for (int e = s, i = 0; e < E; e += 8, ++i)
-                if (!(used >> i & 1) && (bi == 0x7fffffff || L[e] > bv)) { bv = L[e]; bi = e; }
+                if (!(used >> i & 1)) {
+                    // NaN counts as the lowest value: the lanes of a token have to agree on an order, or one of them runs out of
+                    // experts and its index points past the token's logits (the gate weights are NaN all the same)
+                    const float l = L[e], v = l == l ? l : -INFINITY;
+                    if (bi == 0x7fffffff || v > bv) { bv = v; bi = e; }
+                }
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
                 const float ov = __shfl_xor_sync(full, bv, o);
