@@ -1,7 +1,7 @@
 // 4-bit products with few rows per weight matrix: bound by how fast the weights arrive, and below that by the latency of a chain of
 // short kernels.
 //
-// A block owns 128 weight rows of one matrix, the 128-row side of the MMA; the matrix's activation rows are its columns, 32 at a
+// A block (with a long k and few matrices: a cluster, each block a share of k) owns 128 weight rows of one matrix, the 128-row side of the MMA; the matrix's activation rows are its columns, 32 at a
 // time. At its start, before it knows whether and by whom the matrix is used, it asks for all of its weights (up to the shared
 // memory there is: 64 bytes per row and 128 of k), so that every weight of the product is on its way at once. Meanwhile sixteen
 // warps find the matrix's rows in the router's index table (grouped) and bring them in: as values, which they quantise here, or
@@ -11,6 +11,8 @@
 //
 // Warps: 0..15 = rows in, then epilogue (four lane quarters x every fourth group of rows); 16 = TMA of the weights; 17 = MMA issuer, TMEM owner.
 // Every wait is bounded, as in the other kernels.
+#include <algorithm>
+
 #include "launch_pdl.cuh"
 #include "mx_decode.h"
 #include "mx_gemm.cuh"
@@ -47,13 +49,25 @@ __device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {       // the word at this offset of another block of the cluster
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
 // A piece of one row: one k block of 256 elements, 8 per lane, on its way into registers.
 template <int SRC>
 struct Piece {
     static constexpr int kAhead = SRC == kMxSrcF32 ? 2 : SRC == kMxSrcBf16 ? 3 : 6;      // pieces in flight: 16, 12 or 12 registers
     uint4 a, b;
     uint32_t sw;
-    __device__ __forceinline__ void fetch(const MxDecode& p, long row, int kb, int tiles_k, int lane) {
+    __device__ __forceinline__ void fetch(const MxDecode& p, long row, int kb, int tiles_k, int lane) {      // kb: of the whole row
         const int col = kb * kKB + lane * 8;
         a = make_uint4(0, 0, 0, 0); sw = 0;
         if constexpr (SRC == kMxSrcF32) b = a;
@@ -106,7 +120,7 @@ struct Piece {
 // kernel this short arrives from L2 as it runs, so the loop is kept small rather than unrolled. (Handing the k blocks to the
 // MMAs one by one, k block by k block, gained nothing: the pieces then came in as much later as the products ended sooner.)
 template <int SRC>
-__device__ __forceinline__ void rows_in(const MxDecode& p, const uint16_t* list, int r0, int nr, int nkb, uint32_t act, int warp, int lane) {
+__device__ __forceinline__ void rows_in(const MxDecode& p, const uint16_t* list, int r0, int nr, int kb0, int nkb, uint32_t act, int warp, int lane) {
     const int tiles_k = scale_tiles_k(p.k), pieces = nr * nkb;
     // (row, k block) of the piece being stored and of the one being fetched: sixteen pieces further each time
     const int dr = kRowWarps / nkb, dk = kRowWarps - dr * nkb;
@@ -114,7 +128,7 @@ __device__ __forceinline__ void rows_in(const MxDecode& p, const uint16_t* list,
     constexpr int A = Piece<SRC>::kAhead;
     Piece<SRC> x[A];
     auto fetch = [&](Piece<SRC>& d) {
-        if (fu < pieces) d.fetch(p, p.experts ? (int)(list[r0 + fr] * p.src_mul >> 16) : r0 + fr, fk, tiles_k, lane);
+        if (fu < pieces) d.fetch(p, p.experts ? (int)(list[r0 + fr] * p.src_mul >> 16) : r0 + fr, kb0 + fk, tiles_k, lane);
         fu += kRowWarps;
         fr += dr; fk += dk;
         if (fk >= nkb) { fk -= nkb; ++fr; }
@@ -195,7 +209,8 @@ __device__ __forceinline__ int make_list(const MxDecode& p, int e, uint16_t* lis
     return n;
 }
 
-template <int SRC, int EPI>
+// SPLIT: the blocks of a cluster share k.
+template <int SRC, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_constant__ MxDecode p, int stages) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], rows_bar, acc_bar[2], free_bar[2], mma_bar;
@@ -205,8 +220,10 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w_tiles = (p.n + 127) >> 7;
-    const int e = blockIdx.x / w_tiles, w0 = (blockIdx.x % w_tiles) << 7;
-    const int nkb = (p.k + kKB - 1) / kKB;
+    const int split = SPLIT ? p.split : 1, part = SPLIT ? (int)blockIdx.x % split : 0, tile = SPLIT ? (int)blockIdx.x / split : (int)blockIdx.x;
+    const int e = SPLIT ? 0 : tile / w_tiles, w0 = (SPLIT ? tile : tile % w_tiles) << 7;
+    const int nkb_all = (p.k + kKB - 1) / kKB;
+    const int kb0 = SPLIT ? nkb_all * part / split : 0, nkb = SPLIT ? nkb_all * (part + 1) / split - kb0 : nkb_all;      // this block's share of k
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t codes_w = base, act = codes_w + stages * kCodesW, sf_w = act + nkb * kStageA;      // 1024-byte multiples throughout
     volatile int* abort_flag = &abort_s;
@@ -216,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     auto load_stage = [&](int s, int kb) {
         const uint32_t fb = smem_u32(&full_bar[s]);
         mbar_expect_tx(fb, kStageW);
-        tma_load_2d(codes_w + s * kCodesW, map, fb, kb * 128, w0);
-        tma_load_3d(sf_w + s * kSfW, sf_map, fb, 0, 2 * kb, w0 >> 7);
+        tma_load_2d(codes_w + s * kCodesW, map, fb, (kb0 + kb) * 128, w0);
+        tma_load_3d(sf_w + s * kSfW, sf_map, fb, 0, 2 * (kb0 + kb), w0 >> 7);
     };
     // Weights depend on no earlier kernel of the step. With fewer assignments than experts most blocks would ask in vain: they wait.
     const bool ahead = p.experts == 0 || p.n_asg >= p.experts;
@@ -296,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
                         scale_copy(sf_at + a * 4, scale_desc(stage_a + kCodesA + a * kScaleTile));
                     }
                     const uint64_t dw = make_desc(codes_w + s * kCodesW, false, 0), da = make_desc(stage_a, false, 0);
-                    const int steps = (p.k - kb * kKB) / 64;
+                    const int steps = (p.k - (kb0 + kb) * kKB) / 64;
                     auto step = [&](int j) {
                         mma(tmem_base + (ps & 1) * kRows, dw + (uint64_t)(j * 2), da + (uint64_t)(j * 2), idesc | mxf4_ids((j & 1) * 2),
                             sfw_at + (j >> 1) * 4, sf_at + (j >> 1) * 4, (kb | j) != 0);
@@ -321,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
             const int r0 = ps * kRows, nr = min(kRows, count - r0);
             if (ps > 0) ok = __all_sync(kFull, mbar_wait(smem_u32(&mma_bar), (ps - 1) & 1, abort_flag, p.status));      // the last pass's rows have been read
             if (!ok) break;
-            rows_in<SRC>(p, list, r0, nr, nkb, act, warp, lane);
+            rows_in<SRC>(p, list, r0, nr, kb0, nkb, act, warp, lane);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&rows_bar));
@@ -329,7 +346,14 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
             if (!ok) break;
             tc_fence_after();
             const int quarter = warp & 3, set = warp >> 2;
-            drain<EPI>(p, list, r0, nr, tmem_base + ((uint32_t)(quarter * 32) << 16) + (ps & 1) * kRows, set, w0 + quarter * 32 + lane, lane);
+            if constexpr (SPLIT) {                   // this share of the sums, for the cluster (the weights of stage 0 have been read)
+                for (int g = set * 4; g < nr; g += kRowWarps) {
+                    uint32_t v[4];
+                    tmem_ld4(tmem_base + ((uint32_t)(quarter * 32) << 16) + (ps & 1) * kRows + g, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st_shared4(codes_w + (g + i) * 512 + (quarter * 32 + lane) * 4, v[i]);
+                }
+            } else drain<EPI>(p, list, r0, nr, tmem_base + ((uint32_t)(quarter * 32) << 16) + (ps & 1) * kRows, set, w0 + quarter * 32 + lane, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&free_bar[ps & 1]));
@@ -337,6 +361,22 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (SPLIT) {
+        // Row r is added up by the block r % split, its shares in the order of k. Every thread of every block comes by here, also
+        // after a wait that ran out.
+        cluster_sync();
+        if (warp < kRowWarps && w0 + (int)(threadIdx.x & 127) < p.n)
+            for (int r = part + split * (int)(threadIdx.x >> 7); r < p.rows; r += split * (kRowWarps / 4)) {
+                const uint32_t at = codes_w + r * 512 + (threadIdx.x & 127) * 4;
+                float x = 0.0f;
+                for (int q = 0; q < split; ++q) x += ld_cluster(at, q);
+                const size_t to = (size_t)r * p.n + w0 + (threadIdx.x & 127);
+                if constexpr (EPI == kMxF32) static_cast<float*>(p.out)[to] = x;
+                else static_cast<uint16_t*>(p.out)[to] = f2bf(x);
+            }
+        __syncwarp();
+        cluster_sync();            // the others have read this block's share
+    }
     if (warp == kTmaWarp && lane == 0) {
         // No copy may still be on its way into this block's shared memory. The MMA warp has waited for all of them, but in a block
         // without rows, or when a wait ran out: wait (bounded) for the last load of every stage.
@@ -352,31 +392,68 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     }
 }
 
-template <int SRC, int EPI>
+template <int SRC, int EPI, bool SPLIT>
 cudaError_t launch_t(const MxDecode& p, cudaStream_t stream) {
-    const int nkb = (p.k + kKB - 1) / kKB;
+    const int nkb = ((p.k + kKB - 1) / kKB + p.split - 1) / p.split;      // the largest share
     const int room = (kSmemMax - 1024 - nkb * kStageA) / kStageW;
     const int stages = room < nkb ? (room < kMaxStages ? room : kMaxStages) : (nkb < kMaxStages ? nkb : kMaxStages);
     const size_t smem = 1024 + (size_t)nkb * kStageA + (size_t)stages * kStageW;
-    cudaError_t e = cudaFuncSetAttribute(mx_decode_kernel<SRC, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    const auto kernel = mx_decode_kernel<SRC, EPI, SPLIT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return e;
-    const int blocks = ((p.n + 127) / 128) * (p.experts ? p.experts : 1);
-    return launch_pdl(mx_decode_kernel<SRC, EPI>, dim3(blocks), dim3(kThreads), smem, stream, p, stages);
+    const int blocks = ((p.n + 127) / 128) * (p.experts ? p.experts : p.split);
+    if constexpr (!SPLIT) return launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, stream, p, stages);
+    // a cluster per tile, launched the ordinary way (see mx_gemm_2cta.cu)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p, stages);
 }
 template <int SRC>
 cudaError_t launch_dense(const MxDecode& p, cudaStream_t stream) {
-    return p.epi == kMxF32 ? launch_t<SRC, kMxF32>(p, stream) : launch_t<SRC, kMxBf16>(p, stream);
+    if (p.split > 1) return p.epi == kMxF32 ? launch_t<SRC, kMxF32, true>(p, stream) : launch_t<SRC, kMxBf16, true>(p, stream);
+    return p.epi == kMxF32 ? launch_t<SRC, kMxF32, false>(p, stream) : launch_t<SRC, kMxBf16, false>(p, stream);
 }
 
 }  // namespace
 
-bool mx_decode_form(long rows, int groups, int k) {
-    return rows <= kMxDecodeMaxAsg && rows <= (long)kMxDecodeRows * groups && k <= kMxDecodeMaxK;
+// A block alone takes k in turn, about 1.6 us per 1024 of it: from 2048 on a cluster shares it, as far as there are SMs. 1 row, us:
+//     n x k        alone  shared               n x k        alone  shared
+//     2048 x 2048    6.0     5.7               4096 x 4096    9.9     6.5
+//     1024 x 4096    9.8     5.7               1024 x 8192   15.8     6.4
+// Below 2048 the early start of an ordinary launch, which clusters go without, is worth more (1024 x 1024: 4.1 alone, 4.9 shared).
+int mx_decode_split(int n, int k, int num_sms) {
+    const int tiles = (n + 127) / 128, nkb = (k + kKB - 1) / kKB;
+    int split = 1;
+    while (split < 8 && nkb >= 8 && 4 * split <= nkb && 2 * split * tiles <= num_sms) split *= 2;
+    return split;
+}
+
+// Every block brings all rows in for itself, so its time grows with them, where quantising once and 128 x 128 tiles cost the same
+// for 1 row as for 128. Dense layers, us, few rows (8, 16, 24, 32) | tiles:
+//     1024 x 1024   5.0   6.0   7.0   7.9 |  6.4         1024 x 4096   5.9   6.6   7.1   7.6 | 10.4
+//     2048 x 2048   5.9   6.6   7.3   7.7 |  7.8         4096 x 4096   7.1   8.2   9.4  10.4 | 10.6
+//     of codes: 1024 x 1024   4.8   5.5   6.2   6.9 | 4.8        4096 x 4096   7.0   7.8   8.6   9.4 | 9.1
+bool mx_decode_dense(long rows, int k, int split, bool codes) {
+    if (k > kMxDecodeMaxK) return false;
+    const long most = split > 1 ? kMxDecodeRows : std::min<long>(kMxDecodeRows, 16384 / k);
+    return rows <= std::max(1L, codes ? most / 2 : most);
+}
+
+// Experts, us for the whole pass, this kernel | scan, dispatch and tiles, by rows per expert:
+//     16 experts 1024 -> 2048:   8 rows 29.4 | 41.1    16 rows 39.3 | 46.1    32 rows 56.4 | 46.1
+//      4 experts  512 -> 1024:   8 rows 22.6 | 27.3    32 rows 31.7 | 27.4
+bool mx_decode_grouped(long rows, int groups, int k) {
+    return rows <= kMxDecodeMaxAsg && k <= kMxDecodeMaxK && rows <= 16L * groups && rows * k <= 32768L * groups;
 }
 
 cudaError_t launch_mx_decode(const MxDecode& p, cudaStream_t stream) {
-    if (p.epi == kMxUp) return launch_t<kMxSrcBf16, kMxUp>(p, stream);
-    if (p.epi == kMxDown) return launch_t<kMxSrcRows, kMxDown>(p, stream);
+    if (p.epi == kMxUp) return launch_t<kMxSrcBf16, kMxUp, false>(p, stream);
+    if (p.epi == kMxDown) return launch_t<kMxSrcRows, kMxDown, false>(p, stream);
     switch (p.src_kind) {
         case kMxSrcBf16: return launch_dense<kMxSrcBf16>(p, stream);
         case kMxSrcF32: return launch_dense<kMxSrcF32>(p, stream);

@@ -22,6 +22,7 @@ struct MxDecode {
     int rows;                          // dense: rows
     const int* idx; int n_asg; int experts;      // grouped: expert of every assignment (experts = 0: dense)
     int n, k;
+    int split;                         // dense: blocks (a cluster) that share k; grouped: 1
     int epi;                           // MxEpilogue; kMxUp: out_scales row-major as kMxSrcRows; grouped outputs: one row per assignment
     void* out; uint8_t* out_scales;
     const float* gate;                 // kMxDown: per assignment
@@ -35,8 +36,11 @@ inline unsigned mx_row_factor(int divisor) { return (65536u + (unsigned)divisor 
 constexpr int kMxDecodeRows = 32;      // rows per pass
 constexpr int kMxDecodeMaxAsg = 2048, kMxDecodeMaxK = 8192;
 
-// Up to kMxDecodeMaxAsg assignments, kMxDecodeMaxK columns, 32 rows per matrix on average.
-bool mx_decode_form(long rows, int groups, int k);
+// Dense: the number of blocks that share k, and whether this kernel takes the product (codes: the rows come as codes).
+int mx_decode_split(int n, int k, int num_sms);
+bool mx_decode_dense(long rows, int k, int split, bool codes);
+// Grouped: whether this kernel takes both products of the experts; k: the longer of their two.
+bool mx_decode_grouped(long rows, int groups, int k);
 cudaError_t launch_mx_decode(const MxDecode& p, cudaStream_t stream);
 
 }  // namespace tmt

@@ -39,7 +39,7 @@ struct MxGemm {
 // Forms of the product: one CTA per 128 x 128 tile; CTA pairs on 256 x 256 tiles.
 enum MxForm : int { kMxMany = 0, kMxPair = 1 };
 // The form for `rows` activation rows in `groups` groups of about equal size, n outputs; pad: rows that group starts are multiples of.
-int mx_form(long rows, int groups, int n, int num_sms, int pad);
+int mx_form(long rows, int groups, int n, int k, int num_sms, int pad);
 
 // 128-row boxes for the codes of both operands; 128-row bands per box of the scale maps (pair form).
 constexpr int kMxBoxRows = 128;

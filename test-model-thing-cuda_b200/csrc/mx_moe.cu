@@ -252,11 +252,11 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     h->dims.T = tokens;
     h->last_tokens = tokens;
     route_only(h, static_cast<const uint16_t*>(X), Wr);
-    if (mx_decode_form((long)tokens * K, E, std::max(D, H))) {
+    if (mx_decode_grouped((long)tokens * K, E, std::max(D, H))) {
         // Few rows per expert: no dispatch; up finds and quantises its rows itself and writes one row per assignment, down reads those.
         MxDecode q;
         memset(&q, 0, sizeof q);
-        q.idx = h->rb.idx; q.n_asg = tokens * K; q.experts = E; q.status = h->rb.status; q.early = true;
+        q.idx = h->rb.idx; q.n_asg = tokens * K; q.experts = E; q.status = h->rb.status; q.early = true; q.split = 1;
         q.src = X; q.src_kind = kMxSrcBf16; q.src_mul = mx_row_factor(K);
         q.w_maps = m.tables + (size_t)kTabCodes * E; q.w_sf_maps = m.tables + (size_t)kTabScales1 * E;
         q.n = H; q.k = D; q.epi = kMxUp; q.out = m.h_codes; q.out_scales = m.h_scales;
@@ -289,13 +289,13 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
         p.w_scales_tab = m.scale_tab + (size_t)product * E;
     };
     p.n = H; p.k = D; p.epi = kMxUp; p.out = m.h_codes; p.out_scales = m.h_scales;
-    p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
+    p.form = mx_form((long)tokens * K, E, p.n, p.k, h->num_sms, h->pad);
     p.act = m.x_map; p.act_scales = m.x_scales; p.act_sf = m.x_sf;
     weights(0);
     prof_mark(h, kPhGemmUp);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
     p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
-    p.form = mx_form((long)tokens * K, E, p.n, h->num_sms, h->pad);
+    p.form = mx_form((long)tokens * K, E, p.n, p.k, h->num_sms, h->pad);
     p.act = m.h_map; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
     weights(1);
     prof_mark(h, kPhGemmDown);
@@ -321,18 +321,19 @@ void few_rows(const void* src, const void* scales, int kind, int rows, const tmt
     mx_make_scale_map(&p.w_sf, W.scales, W.rows, W.cols, 1);
     p.src = src; p.src_scales = static_cast<const uint8_t*>(scales); p.src_kind = kind;
     p.rows = rows; p.n = W.rows; p.k = W.cols;
+    p.split = mx_decode_split(W.rows, W.cols, sm_count());
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
     cuda_ok(launch_mx_decode(p, s), "matmul_mxfp4 launch");
 }
 
 void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
-    if (mx_decode_form(rows, 1, W.cols)) return few_rows(codes, scales, kMxSrcTiles, rows, W, Y, dtype, status, s);
+    if (mx_decode_dense(rows, W.cols, mx_decode_split(W.rows, W.cols, sm_count()), true)) return few_rows(codes, scales, kMxSrcTiles, rows, W, Y, dtype, status, s);
     MxGemm p;
     memset(&p, 0, sizeof p);
     const int sms = sm_count();
     p.rows = rows; p.n = W.rows; p.k = W.cols;
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
-    p.form = mx_form(rows, 1, p.n, sms, 256);
+    p.form = mx_form(rows, 1, p.n, p.k, sms, 256);
     p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
     mx_make_map(&p.act, codes, rows, p.k, kMxBoxRows);
     mx_make_map(&p.w, W.codes, p.n, p.k, kMxBoxRows);
@@ -387,7 +388,7 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         check_tensors({X, W->codes, W->scales, Y, work});
         if (status) check_tensors({status}, 4);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (mx_decode_form(rows, 1, W->cols)) {
+        if (mx_decode_dense(rows, W->cols, mx_decode_split(W->rows, W->cols, sm_count()), false)) {
             few_rows(X, nullptr, x_dtype == TMT_MOE_F32 ? kMxSrcF32 : kMxSrcBf16, rows, *W, Y, y_dtype, status, s);
             return 0;
         }

@@ -6,7 +6,7 @@ import torch
 
 import mx_ref as R
 import tmt_moe_b200 as M
-from test_gpu_mx import FMT8, exact64, experts_ref, ln_backward_ref, quantized, to_device
+from test_gpu_mx import FMT8, exact64, experts_case, experts_ref, ln_backward_ref, quantized, to_device
 
 pytestmark = pytest.mark.gpu
 
@@ -435,3 +435,42 @@ def test_a_product_whose_output_passes_32_bits():
     few = Layer(5, n, k, 5)
     few.X.copy_(layer.X[probe])
     assert torch.equal(layer.Y[probe], few.run())
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,n,k", [(1, 1024, 4096), (2, 8, 8192), (3, 264, 2112), (5, 2504, 1792), (7, 4104, 4096), (16, 128, 2048), (31, 520, 1856), (32, 1024, 4096)])
+def test_few_rows_against_a_long_k(rows, n, k, out):
+    layer = Layer(rows, n, k, rows, out=out)
+    layer.Y = torch.full((rows + 1, n), 7.0, dtype=out, device="cuda")[:rows]
+    got = layer.run().clone()
+    c, s, _, _ = layer.W._keep[0]
+    wv = torch.empty(n, k, device="cuda")
+    M.dequantize_mxfp4(c, s, wv)
+    a, w = R.q(exact64(layer.X), "e2m1"), exact64(wv)
+    want, tol = a @ w.T, k * 2.0 ** -23 * (np.abs(a) @ np.abs(w).T)        # additions in fp32, then one rounding
+    tol = tol + (2.0 ** -8 * np.abs(want) if out == torch.bfloat16 else 0)
+    assert (np.abs(exact64(got) - want) <= tol * 1.01).all()
+    for _ in range(3):
+        assert torch.equal(layer.run(), got)
+    assert (layer.Y._base[rows] == 7).all()
+    # the product of the same codes
+    codes, scales, Y = raw(rows * k // 2), raw(M.mxfp4_scale_bytes(rows, k)), torch.empty_like(got)
+    M.quantize_mxfp4(layer.X, codes, scales)
+    M.matmul_mxfp4(codes, scales, layer.W, Y)
+    assert torch.equal(Y, got)
+
+
+@pytest.mark.parametrize("T,D,H,E,K", [(60, 256, 512, 16, 2), (100, 192, 64, 13, 1), (40, 5120, 64, 16, 2), (25, 64, 4224, 16, 2), (2000, 192, 128, 8, 2)])
+def test_most_tokens_pick_the_same_expert(T, D, H, E, K):
+    """One expert has most of the rows, more than a pass of the few-row product takes, the others few or none."""
+    x, wr, up, down = experts_case(T, D, H, E, K, T)
+    x[:, 0], wr[:, 0], wr[E - 1, 0] = 4.0, 0.0, 2.0
+    X, Wr, Y = to_device(x, "bf16"), to_device(wr, "bf16"), torch.zeros(T, D, device="cuda").bfloat16()
+    moe = M.MoE(T, D, E, K, hidden=H, training=False)
+    moe.forward_mxfp4(X, Wr, quantized(up), quantized(down), Y, 0.0)
+    assert moe.device_status() == 0
+    idx, w = moe.read("idx"), moe.read("w").astype(np.float64)
+    # the other logits have a deviation of about 0.05 sqrt(D): at the longest rows some of them pass this expert's 8
+    assert (idx[:, 0] == E - 1).mean() > 0.5
+    y, mag = experts_ref(x, up, down, idx, w)
+    assert np.linalg.norm(exact64(Y) - y) <= 2.0 ** -8 * np.linalg.norm(np.abs(y) + mag)
