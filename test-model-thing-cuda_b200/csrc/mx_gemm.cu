@@ -11,7 +11,8 @@
 // tensor memory, 4 columns per tile; the MMA reads two of the four blocks, picked by the scale ids of its descriptor. An MMA and
 // the copies issued before it by the same thread run in order, so the scale columns need no second buffer.
 //
-// Warps: 0 = TMA producer of P, 1 = MMA issuer and TMEM owner, 2..5 = epilogue, 6 = TMA producer of Q. Persistent over tiles,
+// Warps: 0 = TMA producer of P, 1 = MMA issuer and TMEM owner, 2..9 = epilogue (two groups of four, 64 outputs each), 10 = TMA producer of Q.
+// Persistent over tiles,
 // two accumulators in tensor memory. Every wait is bounded, as in the bf16 kernels.
 #include <stdexcept>
 #include <string>
@@ -25,15 +26,16 @@ namespace {
 using namespace mxg;
 
 constexpr int kBP = 128;                 // rows of a tile on the P side
-constexpr int kThreads = 224;
+constexpr int kThreads = 352;
+constexpr int kOutBox = 32 * 128;        // staged outputs of a warp: its 32 rows x 128 bytes
 
 template <int BN> struct Shape {
     static constexpr int kQBands = (BN + 127) / 128;                     // 128-row bands of scale tiles on the Q side
     static constexpr int kCodesP = kBP * 128, kCodesQ = BN * 128;
     static constexpr int kSfP = 2 * kScaleTile, kSfQ = 2 * kScaleTile * kQBands;
     static constexpr int kStageBytes = kCodesP + kCodesQ + kSfP + kSfQ;
-    static constexpr int kStages = (200 * 1024) / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr int kStages = (220 * 1024 - 8 * kOutBox) / kStageBytes;
+    static constexpr int kSmem = kStages * kStageBytes + 8 * kOutBox + 1024;
     static constexpr uint32_t kSfCol = 2 * BN;                           // scale columns follow the two accumulators
     static constexpr uint32_t kCols = 2 * BN + 8 + 8 * kQBands <= 128 ? 128 : 2 * BN + 8 + 8 * kQBands <= 256 ? 256 : 512;
     static_assert(2 * BN + 8 + 8 * kQBands <= 512, "tensor memory has 512 columns");
@@ -54,57 +56,69 @@ __device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t dp, uint64_t 
         ::"r"(tmem_d), "l"(dp), "l"(dq), "r"(idesc), "r"(sfp), "r"(sfq), "r"(accumulate) : "memory");
 }
 
-// ---- epilogues of one warp: its 32 TMEM lanes, all columns of the tile ----
-
-// 32 neighbouring outputs of one activation row (kMxUp: after the silu). `word` collects the scale bytes of 4 blocks.
-template <int EPI>
-__device__ __forceinline__ void drain_chunk(const MxGemm& p, long row, int col0, float gate, float (&v)[32], uint32_t& word) {
-    if constexpr (EPI == kMxUp) {            // one block (n is a multiple of 64 here)
-        uint32_t q[4];
-        const uint32_t sb = quantize32(v, q);
-        stg16(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col0 / 2, make_uint4(q[0], q[1], q[2], q[3]));
-        const int k4 = (col0 >> 5) & 3;
-        word |= sb << (8 * k4);
-        if (k4 == 3 || col0 + 32 >= p.n) {
-            *reinterpret_cast<uint32_t*>(p.out_scales + scale_word(row, col0 >> 7, scale_tiles_k(p.n))) = word;
-            word = 0;
-        }
-    } else if constexpr (EPI == kMxF32) {
-        float* dst = static_cast<float*>(p.out) + row * p.n + col0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (col0 + q * 4 < p.n) *reinterpret_cast<float4*>(dst + q * 4) = make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
-    } else {
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.n + col0;
-        if constexpr (EPI == kMxDown) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= gate;
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (col0 + q * 8 < p.n)
-                stg16(dst + q * 8, make_uint4(pack_bf2(v[q * 8], v[q * 8 + 1]), pack_bf2(v[q * 8 + 2], v[q * 8 + 3]),
-                                              pack_bf2(v[q * 8 + 4], v[q * 8 + 5]), pack_bf2(v[q * 8 + 6], v[q * 8 + 7])));
-    }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
 }
 
-// Many rows: lane = activation row, columns = outputs.
-template <int EPI, int BN>
-__device__ __forceinline__ void drain_rows(const MxGemm& p, const Tile& ti, uint32_t tm, int r) {
-    const long row = (long)ti.row0 + r;
-    const bool row_ok = r < ti.rows;
+// The epilogue of one warp: 32 rows (its TMEM lanes) and 64 of the tile's 128 outputs. The accumulator is handed back once its
+// 64 columns are in registers. Outputs go through 4 KB of shared memory per warp, so that 8 lanes store the 128 bytes of a row
+// together: a lane per row, 16 bytes each into 32 rows, took 1.4 us more for the fp32 outputs of a single turn of tiles.
+template <int EPI>
+__device__ __forceinline__ void drain_tile(const MxGemm& p, const Tile& ti, uint32_t tm, int quarter, int group, uint32_t buf, uint32_t tempty, int lane) {
+    const int row0 = ti.row0 + quarter * 32, rows = ti.rows - quarter * 32, col0 = ti.w0 + group * 64;
+    const long row = (long)row0 + lane;
     float gate = 0.0f;
-    if constexpr (EPI == kMxDown) gate = row_ok ? p.row_scale[row] : 0.0f;
-    uint32_t word = 0;
-#pragma unroll 1
-    for (int cc = 0; cc < BN / 32; ++cc) {
-        const int col0 = ti.w0 + cc * 32;
-        if (col0 >= p.n) break;
-        float v[32];
-        __syncwarp();
-        tmem_ld32(tm + (uint32_t)(cc * 32), v);
-        if constexpr (EPI == kMxUp) silu32(v);
-        if (row_ok) drain_chunk<EPI>(p, row, col0, gate, v, word);
+    if constexpr (EPI == kMxDown) gate = lane < rows ? p.row_scale[row] : 0.0f;
+    uint32_t v[64];
+    tmem_start64(tm + group * 64, v);
+    tmem_wait64(v);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(tempty);
+    if (rows <= 0 || col0 >= p.n) return;
+    if constexpr (EPI == kMxUp) {            // silu, then two blocks of 32: 32 bytes of codes and two scale bytes per row
+        uint32_t scales = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float f[32];
+            uint32_t q[4];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[32 * b + i]);
+            silu32(f);
+            const uint32_t sb = quantize32(f, q);
+            if (lane < rows) stg16(static_cast<uint8_t*>(p.out) + row * (p.n / 2) + col0 / 2 + 16 * b, make_uint4(q[0], q[1], q[2], q[3]));
+            scales |= sb << (8 * b);
+        }
+        if (lane < rows)
+            *reinterpret_cast<uint16_t*>(p.out_scales + scale_word(row, col0 >> 7, scale_tiles_k(p.n)) + ((col0 >> 5) & 3)) = (uint16_t)scales;
+    } else {
+        constexpr int kBytes = EPI == kMxF32 ? 4 : 2, kBoxCols = 128 / kBytes;
+        uint8_t* out = static_cast<uint8_t*>(p.out);
+#pragma unroll
+        for (int x0 = 0; x0 < 64; x0 += kBoxCols) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (EPI == kMxF32) w[i] = v[x0 + 4 * q + i];
+                    else if constexpr (EPI == kMxDown) w[i] = pack_pair(gate * __uint_as_float(v[8 * q + 2 * i]), gate * __uint_as_float(v[8 * q + 2 * i + 1]));
+                    else w[i] = pack_pair(__uint_as_float(v[8 * q + 2 * i]), __uint_as_float(v[8 * q + 2 * i + 1]));
+                }
+                st_shared16(buf + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+            const int c = lane & 7;
+            const bool col_ok = col0 + x0 + c * (16 / kBytes) < p.n;       // n is a multiple of 8: whole 16-byte pieces
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                if (r < rows && col_ok) stg16(out + ((long)(row0 + r) * p.n + col0 + x0) * kBytes + c * 16, lds16(buf + r * 128 + ((c ^ (r & 7)) << 4)));
+            }
+            __syncwarp();
+        }
     }
 }
 
@@ -126,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     if (threadIdx.x == 0) {
         abort_s = 0;
         for (int s = 0; s < S::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&empty_bar[s]), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 4); }
+        for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     const int nkb = (p.k + kKB - 1) / kKB;
     const int tiles_k = scale_tiles_k(p.k);
 
-    if (warp == 0 || warp == 6) {
+    if (warp == 0 || warp == 10) {
         // ---------------- producers: codes box and scale tiles of one operand per stage ----------------
         if (lane == 0) {
             const bool is_p = warp == 0;
@@ -226,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (j < steps) {
-                                                        mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | mxf4_ids((j & 1) * 2), sfp_t + (j >> 1) * 4,
+                            mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | mxf4_ids((j & 1) * 2), sfp_t + (j >> 1) * 4,
                                      sfq_t + (j >> 1) * 4 * S::kQBands, (kb | j) != 0);
                         }
                     tc_commit(smem_u32(&empty_bar[s]));
@@ -242,7 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
         __syncwarp();
     } else {
         // ---------------- epilogue ----------------
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, group = (warp - 2) >> 2;
+        const uint32_t buf = sf_q + S::kStages * S::kSfQ + (uint32_t)(warp - 2) * kOutBox;
         int acc = 0; uint32_t acc_ph = 0;
         for (int t = blockIdx.x;; t += gridDim.x) {
             Tile ti;
@@ -250,10 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[acc]), acc_ph, abort_flag, p.status))) break;
             tc_fence_after();
             const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
-            drain_rows<EPI, BN>(p, ti, tm, quarter * 32 + lane);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+            drain_tile<EPI>(p, ti, tm, quarter, group, buf, smem_u32(&tempty_bar[acc]), lane);
             if (++acc == 2) { acc = 0; acc_ph ^= 1; }
         }
     }
