@@ -11,8 +11,6 @@
 //
 // Warps: 0..15 = rows in, then epilogue (four lane quarters x every fourth group of rows); 16 = TMA of the weights; 17 = MMA issuer, TMEM owner.
 // Every wait is bounded, as in the other kernels.
-#include <algorithm>
-
 #include "launch_pdl.cuh"
 #include "mx_decode.h"
 #include "mx_gemm.cuh"
@@ -415,8 +413,8 @@ cudaError_t launch_t(const MxDecode& p, cudaStream_t stream) {
 }
 template <int SRC>
 cudaError_t launch_dense(const MxDecode& p, cudaStream_t stream) {
-    if (p.split > 1) return p.epi == kMxF32 ? launch_t<SRC, kMxF32, true>(p, stream) : launch_t<SRC, kMxBf16, true>(p, stream);
-    return p.epi == kMxF32 ? launch_t<SRC, kMxF32, false>(p, stream) : launch_t<SRC, kMxBf16, false>(p, stream);
+    if (SRC == kMxSrcTiles || p.split > 1) return p.epi == kMxF32 ? launch_t<SRC, kMxF32, true>(p, stream) : launch_t<SRC, kMxBf16, true>(p, stream);
+    if constexpr (SRC != kMxSrcTiles) return p.epi == kMxF32 ? launch_t<SRC, kMxF32, false>(p, stream) : launch_t<SRC, kMxBf16, false>(p, stream);
 }
 
 }  // namespace
@@ -425,7 +423,7 @@ cudaError_t launch_dense(const MxDecode& p, cudaStream_t stream) {
 //     n x k        alone  shared               n x k        alone  shared
 //     2048 x 2048    6.0     5.7               4096 x 4096    9.9     6.5
 //     1024 x 4096    9.8     5.7               1024 x 8192   15.8     6.4
-// Below 2048 the early start of an ordinary launch, which clusters go without, is worth more (1024 x 1024: 4.1 alone, 4.9 shared).
+// Below 2048 a block alone is done sooner than any cluster was (1024 x 1024: 4.2): it starts early, which clusters go without.
 int mx_decode_split(int n, int k, int num_sms) {
     const int tiles = (n + 127) / 128, nkb = (k + kKB - 1) / kKB;
     int split = 1;
@@ -433,22 +431,27 @@ int mx_decode_split(int n, int k, int num_sms) {
     return split;
 }
 
-// Every block brings all rows in for itself, so its time grows with them, where quantising once and 128 x 128 tiles cost the same
-// for 1 row as for 128. Dense layers, us, few rows (8, 16, 24, 32) | tiles:
-//     1024 x 1024   5.0   6.0   7.0   7.9 |  6.4         1024 x 4096   5.9   6.6   7.1   7.6 | 10.4
-//     2048 x 2048   5.9   6.6   7.3   7.7 |  7.8         4096 x 4096   7.1   8.2   9.4  10.4 | 10.6
-//     of codes: 1024 x 1024   4.8   5.5   6.2   6.9 | 4.8        4096 x 4096   7.0   7.8   8.6   9.4 | 9.1
+// Every block brings all rows in for itself, 0.03 us per row and 256 of its share of k, where quantising once and 128 x 128 tiles
+// cost the same for 1 row as for 128. Dense layers, us, few rows (1, 8, 16, 24, 32) | tiles:
+//      320 -> 4096   3.9   4.1   4.6   5.3   5.8 |  4.9         4096 -> 1024   5.7   5.9   6.5   7.1   7.6 |  9.7
+//     1024 -> 1024   4.3   4.9   6.0   7.1   8.0 |  5.7         4096 -> 4096   6.4   7.1   8.2   9.4  10.4 |  9.8
+//     2048 -> 2048   5.7   5.9   6.6   7.3   7.8 |  7.1         8192 -> 1024   6.4   7.0   8.1   9.1  10.1 | 14.8
+// and of codes, where only a k long enough to be shared pays:
+//     1024 -> 1024   4.4   5.0   5.6   6.3   7.0 |  4.0         4096 -> 4096   6.6   7.0   7.8   8.6   9.3 |  8.3
+//     2048 -> 2048   5.7   6.0   6.5   7.1   7.4 |  5.4         8192 -> 1024   6.4   6.8   7.6   8.3   9.0 | 13.2
 bool mx_decode_dense(long rows, int k, int split, bool codes) {
-    if (k > kMxDecodeMaxK) return false;
-    const long most = split > 1 ? kMxDecodeRows : std::min<long>(kMxDecodeRows, 16384 / k);
-    return rows <= std::max(1L, codes ? most / 2 : most);
+    if (k > kMxDecodeMaxK || rows > kMxDecodeRows) return false;
+    const long nkb = (k + kKB - 1) / kKB, work = rows * ((nkb + split - 1) / split);
+    if (codes) return split > 1 && work <= 8 * nkb - 64;
+    return work <= (split > 1 ? 8 * nkb - 24 : 40);
 }
 
 // Experts, us for the whole pass, this kernel | scan, dispatch and tiles, by rows per expert:
-//     16 experts 1024 -> 2048:   8 rows 29.4 | 41.1    16 rows 39.3 | 46.1    32 rows 56.4 | 46.1
-//      4 experts  512 -> 1024:   8 rows 22.6 | 27.3    32 rows 31.7 | 27.4
+//     16 experts 1024 -> 2048:   2 rows 26.6 | 33.8     8 rows 29.8 | 34.2    16 rows 41.6 | 38.4
+//      4 experts  512 -> 1024:   2 rows 21.2 | 25.5     8 rows 22.1 | 26.4    32 rows 32.1 | 26.3
 bool mx_decode_grouped(long rows, int groups, int k) {
-    return rows <= kMxDecodeMaxAsg && k <= kMxDecodeMaxK && rows <= 16L * groups && rows * k <= 32768L * groups;
+    const long nkb = (k + kKB - 1) / kKB;
+    return rows <= kMxDecodeMaxAsg && k <= kMxDecodeMaxK && rows <= 20L * groups && rows * nkb <= 80L * groups;
 }
 
 cudaError_t launch_mx_decode(const MxDecode& p, cudaStream_t stream) {

@@ -312,17 +312,17 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-// Pairs where the single CTAs' tiles would take more than one turn of the SMs and k is long, or more than two turns.
+// Pairs where the single CTAs' tiles would take more than one turn of the SMs and k is long, or more than three turns.
 // Dense layers, us, single CTAs / pairs by the number of 128 x 128 tiles (148 SMs):
-//     1024 -> 1024    192:  9.4 / 10.0    256:  9.8 / 10.6    384: 13.1 / 13.1    512: 15.7 / 13.7    1024: 26.3 / 21.9
-//     1024 -> 4096    128:  6.8 /  9.1    256:  8.8 /  9.2    384: 11.4 / 11.2    512: 13.7 / 11.3    1024: 20.9 / 16.4
-//     2048 -> 2048     64:  8.2 / 10.1    128:  8.6 / 10.6    192: 12.1 / 11.2    256: 12.9 / 11.8     512: 20.4 / 16.6
-//     4096 -> 1024    128: 13.9 / 15.2    160: 20.1 / 16.3    256: 23.2 / 18.9    512: 41.9 / 32.4
-//     4096 -> 4096    128: 11.8 / 13.0    256: 18.6 / 14.3    384: 25.4 / 20.5   1024: 53.5 / 37.0
+//     1024 -> 1024    256: 10.3 / 10.6    384: 12.1 / 13.2    512: 14.3 / 13.7    1024: 24.3 / 21.9
+//     1024 -> 4096    256:  8.2 /  9.2    384: 10.5 / 11.2    512: 12.3 / 11.4    1024: 19.6 / 16.5
+//     2048 -> 2048    128:  8.2 / 10.7    192: 13.1 / 11.2    256: 13.2 / 11.8     512: 20.0 / 16.5
+//     4096 -> 1024    128: 13.3 / 15.3    160: 19.8 / 16.3    256: 22.6 / 19.0     512: 44.1 / 32.3
+//     4096 -> 4096    128: 11.3 / 13.1    256: 19.0 / 14.3    384: 25.1 / 20.6    1024: 53.7 / 37.2
 int mx_form(long rows, int groups, int n, int k, int num_sms, int pad) {
     const long each = (rows + groups - 1) / groups;
     const long tiles = groups * ((each + 127) / 128) * ((n + 127) / 128);
-    return pad % 256 == 0 && tiles > (k >= 2048 ? 1 : 2) * num_sms ? kMxPair : kMxMany;
+    return pad % 256 == 0 && tiles > (k >= 2048 ? 1 : 3) * num_sms ? kMxPair : kMxMany;
 }
 
 namespace {
