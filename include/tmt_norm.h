@@ -56,7 +56,7 @@ size_t tmt_ln_backward_act8_scratch_bytes(int rows, int dim);
 
 /* The gradient of the LayerNorm with x replaced by the checkpoint's value, and mean and rstd those of the forward pass:
  * xh = (x - mean) * rstd, g = dY * gamma, dX = rstd * (g - sum(g) / dim - xh * (sum(g * xh) / dim)), dGamma = sum over the rows
- * of dY * xh, dBeta = sum of dY. Sums in fp32, in an order fixed by the shape; dX is rounded once to bf16; dGamma and dBeta
+ * of dY * xh, dBeta = sum of dY. rows: at least 1. Sums in fp32, in an order fixed by the shape; dX is rounded once to bf16; dGamma and dBeta
  * are written. A NaN block of the checkpoint gives NaN in its row of dX and in its columns of dGamma. */
 int tmt_ln_backward_act8(const void* codes, const void* scales, int format, const void* dY, const float* gamma, const float* mean,
                          const float* rstd, void* dX, float* dGamma, float* dBeta, int rows, int dim, void* scratch, void* stream);
