@@ -37,7 +37,7 @@ class Layer:
         return self.Y
 
 
-FORMS = [(5, 520, 320), (300, 264, 448), (9500, 512, 64)]          # few rows, some, many
+FORMS = [(5, 520, 320), (3, 264, 2112), (300, 264, 448), (9500, 512, 64)]          # few rows, few against a long k, some, many
 
 
 class Decoder:
@@ -474,3 +474,55 @@ def test_most_tokens_pick_the_same_expert(T, D, H, E, K):
     assert (idx[:, 0] == E - 1).mean() > 0.5
     y, mag = experts_ref(x, up, down, idx, w)
     assert np.linalg.norm(exact64(Y) - y) <= 2.0 ** -8 * np.linalg.norm(np.abs(y) + mag)
+
+
+def test_every_form_recorded_side_by_side_and_replayed():
+    """The layers fork onto two streams inside one recording and join again."""
+    side = [torch.cuda.Stream() for _ in range(2)]
+    layers = [Layer(*f, 40 + i, s.cuda_stream) for s in side for i, f in enumerate(FORMS)]
+    want = [l.run().clone() for l in layers]
+    torch.cuda.synchronize()
+    main, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(main):
+        with torch.cuda.graph(g, stream=main):
+            for s in side:
+                s.wait_stream(main)
+            for _ in range(3):
+                for l in layers:
+                    l.run()
+            for s in side:
+                main.wait_stream(s)
+        for _ in range(5):
+            for l in layers:
+                l.Y.zero_()
+            g.replay()
+            for l, w in zip(layers, want):
+                assert torch.equal(l.Y, w)
+    main.synchronize()
+    del g
+
+
+def test_handles_of_two_streams_at_once():
+    D, H, E, K = 256, 192, 4, 2
+    up, down = M.Mxfp4Weights(quantized(torch.randn(E, H, D).numpy() * 0.05)), M.Mxfp4Weights(quantized(torch.randn(E, D, H).numpy() * 0.05))
+    Wr = bf((E, D), 2, 0.05)
+    runs = []
+    for i, T in enumerate((7, 300, 2500, 9)):
+        s = torch.cuda.Stream()
+        moe = M.MoE(T, D, E, K, hidden=H, training=False, stream=s.cuda_stream)
+        runs.append((moe, bf((T, D), 30 + i), torch.zeros(T, D, device="cuda").bfloat16()))
+    torch.cuda.synchronize()
+    want = []
+    for moe, X, Y in runs:
+        moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
+        assert moe.device_status() == 0
+        want.append(Y.clone())
+        torch.cuda.synchronize()
+        Y.zero_()
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for moe, X, Y in runs:
+            moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
+    torch.cuda.synchronize()
+    for (moe, _, Y), w in zip(runs, want):
+        assert moe.device_status() == 0 and torch.equal(Y, w)
