@@ -16,7 +16,7 @@ enum MxEpilogue : int {
 };
 
 struct MxGemm {
-    CUtensorMap act, w;                 // codes as bytes, 128-byte boxes (mx_act_map / mx_weight_map)
+    CUtensorMap act, w;                 // codes as bytes, 128-byte boxes (mx_make_map)
     const CUtensorMap* w_maps;          // grouped: one map per expert in device memory (then `w` is not used)
     // scale tiles of the activations (group starts are multiples of 128 rows, of 256 for kMxPair) and of the weights
     const uint8_t* act_scales;          // kMxMany

@@ -19,6 +19,10 @@
 // four, two runs of 64 columns each), 10 = TMA of weight codes, 11 = TMA of scales (a TMA instruction keeps its warp busy for some
 // 200 clocks). An epilogue thread owns a row: it loads 64 columns, hands them back, and works from registers; outputs are staged
 // in shared memory and written by TMA stores.
+// Measured (1 TF/s = 10^12 FLOP/s; operands of random codes): 16384 x 8192 -> 8192 5350 TF/s, held by the power limit at 1.3 to 1.4 GHz (7530 TF/s
+// on zeros, at 1.965 GHz: 640 clocks per k block of 512 ideal); 65536 x 2048 -> 2048 118 us = 4660 TF/s; 16384 x 1024 -> 4096 36 us = 3800 TF/s,
+// 4000 clocks per tile of 2048 ideal: some 500 between the last product of a tile and the first of the next, the rest waits
+// for operands while the outputs (64 KB a tile and CTA) leave through the same L2 (without the stores: 33 us).
 // Waits are bounded as in the bf16 kernels; both CTAs always reach the closing cluster barrier before tensor memory is freed.
 #include "mx_gemm.cuh"
 

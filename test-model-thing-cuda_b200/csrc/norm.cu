@@ -36,105 +36,108 @@ __device__ __forceinline__ float butterfly(float v) {
     return v;
 }
 
-// One warp per row (rows taken grid-stride), R rows at a time: they stay in registers between the statistics and the output (one
-// read of X), their reductions overlap, and gamma and beta are loaded once for all of them.
+// One warp per row (rows taken grid-stride); the row stays in registers between the statistics and the output (one
+// read of X) and the next row is fetched before the current one is reduced.
 // FMT: mx::kE4M3 / mx::kE5M2 leaves an 8-bit checkpoint of the row as well (a block of 32 is the vectors of 4 neighbouring
 // lanes): one byte more per element written, and no second read of X. 0: none.
-// Bound: HBM; at 131072 x 2048 177 us without a checkpoint (6.1 TB/s; one row at a time, the next one on its way in registers: 196) and 243
-// with one (5.6 TB/s). There two rows want more registers than three blocks an SM leave (264 at two blocks, 321 without a
-// limit), four blocks spill (390), and storing the scale bytes of a row together instead of 8 at a time gains nothing (243).
-template <int NV, int R, int FMT>
-__global__ void __launch_bounds__(kFwdWarps * 32, FMT != 0 && NV <= 8 ? 3 : 0) ln_fwd_kernel(const uint16_t* __restrict__ X, const float* __restrict__ gamma,
+// Bound: HBM; 131072 x 2048 takes 196 us without a checkpoint (5.5 TB/s) and 251 with one (5.4), 131072 x 1024 100 and 126. Several rows a
+// warp without the fetch ahead: 175 and 246 at 2048, but 10.6 and 17.0 instead of 8.8 and 11.6 at 8000 x 1024; the codes
+// packed in the first pass, next to the sums: 291 at 2048 (registers).
+template <int NV, int FMT>
+__global__ void __launch_bounds__(kFwdWarps * 32) ln_fwd_kernel(const uint16_t* __restrict__ X, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, uint16_t* __restrict__ Y,
                                                                 float* __restrict__ mean, float* __restrict__ rstd, int rows, int D,
                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     const int lane = threadIdx.x & 31;
     const int nvec = D >> 3;
     const long stride = (long)gridDim.x * kFwdWarps;
+    long r = (long)blockIdx.x * kFwdWarps + (threadIdx.x >> 5);
+    if (r >= rows) return;
     const float fd = (float)D;
-    for (long r0 = (long)blockIdx.x * kFwdWarps + (threadIdx.x >> 5); r0 < rows; r0 += R * stride) {
-        uint4 raw[R][NV];
+    constexpr bool kPrefetch = NV <= 8;              // wider rows would not fit two copies in registers
+    uint4 raw[NV], nxt[kPrefetch ? NV : 1];
+    auto fetch = [&](long row, auto& dst) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const long row = min(r0 + j * stride, (long)rows - 1);      // past the end: a valid row, not written
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int v = lane + i * 32;
-                if (v < nvec) raw[j][i] = ldg16(X + row * D + v * 8);
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int v = lane + i * 32;
+            if (v < nvec) dst[i] = ldg16(X + row * D + v * 8);
         }
-        float m[R], rs[R];
+    };
+    if constexpr (kPrefetch) fetch(r, raw);
+    for (; r < rows; r += stride) {
+        if constexpr (kPrefetch) {
+            if (r + stride < rows) fetch(r + stride, nxt);  // the next row travels while this one is reduced and written
+        } else {
+            fetch(r, raw);
+        }
+        float sum = 0.0f, sq = 0.0f;
+        uint32_t amax[FMT != 0 ? NV : 1];                // largest magnitude of a lane's vector (bf16 magnitudes order like their bits)
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const long r = r0 + j * stride;
-            float sum = 0.0f, sq = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int v = lane + i * 32;
-                if (v >= nvec) continue;                 // dim is a multiple of 32 where FMT != 0: the four lanes of a block agree
-                const uint4& x = raw[j][i];
+        for (int i = 0; i < NV; ++i) {
+            const int v = lane + i * 32;
+            if (FMT != 0) amax[FMT != 0 ? i : 0] = 0;
+            if (v < nvec) {
                 float f[8];
-                unpack8(x, f);
+                unpack8(raw[i], f);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) { sum = __fadd_rn(sum, f[q]); sq = __fmaf_rn(f[q], f[q], sq); }
-                if constexpr (FMT != 0) {                // the checkpoint needs no statistics: from the same unpacked elements
-                    uint32_t a = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-                    a = max(a >> 16, a & 0xffffu) << 16;                 // bf16 magnitudes order like their bits
-                    const unsigned block = 0xfu << (lane & 28);
-                    a = max(a, __shfl_xor_sync(block, a, 1));
-                    a = max(a, __shfl_xor_sync(block, a, 2));
+                if constexpr (FMT != 0) {
+                    const uint32_t m = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+                    amax[i] = max(m >> 16, m & 0xffffu) << 16;
+                }
+            }
+        }
+        sum = butterfly(sum);
+        sq = butterfly(sq);
+        const float m = __fdiv_rn(sum, fd);
+        const float var = __fsub_rn(__fdiv_rn(sq, fd), __fmul_rn(m, m));
+        const float rs = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(var, kEps)));
+        if (lane == 0) { mean[r] = m; rstd[r] = rs; }
+        uint16_t* y = Y + r * D;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = lane + i * 32;
+            if (v < nvec) {
+                float f[8];
+                unpack8(raw[i], f);
+                const float4 g0 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8)), g1 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8) + 1);
+                const float4 b0 = __ldg(reinterpret_cast<const float4*>(beta + v * 8)), b1 = __ldg(reinterpret_cast<const float4*>(beta + v * 8) + 1);
+                // packed pairs: each half is the scalar operation, rounded to nearest, so the bits are those stated in the header
+                const float2 gg[4] = {make_float2(g0.x, g0.y), make_float2(g0.z, g0.w), make_float2(g1.x, g1.y), make_float2(g1.z, g1.w)};
+                const float2 bb[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y), make_float2(b1.z, b1.w)};
+                const float2 nm = make_float2(-m, -m), r2 = make_float2(rs, rs);
+                uint32_t o[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 t = __ffma2_rn(__fmul2_rn(__fadd2_rn(make_float2(f[2 * q], f[2 * q + 1]), nm), r2), gg[q], bb[q]);
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[q]) : "f"(t.y), "f"(t.x));
+                }
+                stg16(y + v * 8, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+            if constexpr (FMT != 0) {                    // dim is a multiple of 32: the four lanes of a block agree on v < nvec
+                uint32_t a = amax[i];
+                a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                if (v < nvec) {
                     const uint32_t sb = mx::scale_byte<FMT>(a);
-                    const float2 i2 = make_float2(mx::inv_scale(sb), mx::inv_scale(sb));
+                    const float inv = mx::inv_scale(sb);
+                    float f[8];
+                    unpack8(raw[i], f);
+                    const float2 i2 = make_float2(inv, inv);
                     float2 p[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) p[q] = __fmul2_rn(make_float2(f[2 * q], f[2 * q + 1]), i2);
                     uint32_t lo = mx::pack_f8x4<FMT>(p[0].x, p[0].y, p[1].x, p[1].y);
                     uint32_t hi = mx::pack_f8x4<FMT>(p[2].x, p[2].y, p[3].x, p[3].y);
                     if (sb == 255u) { lo = 0; hi = 0; }
-                    if (r < rows) {
-                        *reinterpret_cast<uint2*>(codes + r * D + v * 8) = make_uint2(lo, hi);
-                        if ((lane & 3) == 0) scales[r * (D >> 5) + (v >> 2)] = (uint8_t)sb;
-                    }
+                    *reinterpret_cast<uint2*>(codes + r * D + v * 8) = make_uint2(lo, hi);
+                    if ((lane & 3) == 0) scales[r * (D >> 5) + (v >> 2)] = (uint8_t)sb;
                 }
             }
-            m[j] = sum; rs[j] = sq;
         }
+        if constexpr (kPrefetch) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            m[j] = __fdiv_rn(butterfly(m[j]), fd);
-            const float var = __fsub_rn(__fdiv_rn(butterfly(rs[j]), fd), __fmul_rn(m[j], m[j]));
-            rs[j] = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(var, kEps)));
-            const long r = r0 + j * stride;
-            if (lane == 0 && r < rows) { mean[r] = m[j]; rstd[r] = rs[j]; }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int v = lane + i * 32;
-            // packed pairs: each half is the scalar operation, rounded to nearest, so the bits are those stated in the header
-            float2 gg[4], bb[4];
-            if (v < nvec) {
-                const float4 g0 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8)), g1 = __ldg(reinterpret_cast<const float4*>(gamma + v * 8) + 1);
-                const float4 b0 = __ldg(reinterpret_cast<const float4*>(beta + v * 8)), b1 = __ldg(reinterpret_cast<const float4*>(beta + v * 8) + 1);
-                gg[0] = make_float2(g0.x, g0.y); gg[1] = make_float2(g0.z, g0.w); gg[2] = make_float2(g1.x, g1.y); gg[3] = make_float2(g1.z, g1.w);
-                bb[0] = make_float2(b0.x, b0.y); bb[1] = make_float2(b0.z, b0.w); bb[2] = make_float2(b1.x, b1.y); bb[3] = make_float2(b1.z, b1.w);
-            }
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                const long r = r0 + j * stride;
-                const bool ok = v < nvec && r < rows;
-                float f[8];
-                unpack8(raw[j][i], f);
-                if (ok) {
-                    const float2 nm = make_float2(-m[j], -m[j]), r2 = make_float2(rs[j], rs[j]);
-                    uint32_t o[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 t = __ffma2_rn(__fmul2_rn(__fadd2_rn(make_float2(f[2 * q], f[2 * q + 1]), nm), r2), gg[q], bb[q]);
-                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[q]) : "f"(t.y), "f"(t.x));
-                    }
-                    stg16(Y + r * D + v * 8, make_uint4(o[0], o[1], o[2], o[3]));
-                }
-            }
+            for (int i = 0; i < NV; ++i) raw[i] = nxt[i];
         }
     }
 }
@@ -347,11 +350,11 @@ void launch_ln_fwd(const void* X, const float* gamma, const float* beta, void* Y
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint16_t* x = static_cast<const uint16_t*>(X);
     uint16_t* y = static_cast<uint16_t*>(Y);
-    if (nv <= 2) ln_fwd_kernel<2, 4, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
-    else if (nv <= 4) ln_fwd_kernel<4, 2, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
-    else if (nv <= 8) ln_fwd_kernel<8, FMT == 0 ? 2 : 1, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
-    else if (nv <= 16) ln_fwd_kernel<16, 1, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
-    else ln_fwd_kernel<kFwdMaxVec, 1, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    if (nv <= 2) ln_fwd_kernel<2, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 4) ln_fwd_kernel<4, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 8) ln_fwd_kernel<8, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else if (nv <= 16) ln_fwd_kernel<16, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
+    else ln_fwd_kernel<kFwdMaxVec, FMT><<<grid, block, 0, s>>>(x, gamma, beta, y, mean, rstd, rows, dim, codes, scales);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw std::runtime_error(std::string("LayerNorm forward launch failed: ") + cudaGetErrorString(e));
 }
