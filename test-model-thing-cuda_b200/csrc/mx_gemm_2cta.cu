@@ -112,6 +112,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    __syncwarp();
+    cluster_sync();            // the pair's allocation is one act of both CTAs: both are there, with their barriers, before it
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -119,7 +121,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
     load_groups<2 * kRows>(p, groups);
     tc_fence_before();
     __syncthreads();
-    cluster_sync();            // both CTAs' barriers are initialised and both hold their tensor memory
+    cluster_sync();            // both hold their tensor memory
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
     const int w_tiles = (p.n + kCols - 1) / kCols;
@@ -313,15 +315,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
     }
+    __syncthreads();
+    // Neither leaves before both have freed theirs: without this barrier and the one before the allocation, about one launch in 40000 of a
+    // busy queue stood still, one CTA inside its allocation, the other waiting for it.
+    cluster_sync();
 }
 
 template <int EPI>
 cudaError_t launch_t(const MxGemm& p, int grid, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(mx_gemm_2cta_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    // An ordinary launch: no part in the programmatic chains of the short kernels. With the early start on both sides (the quantiser
-    // of the next call resident and waiting while this kernel's clusters ran), a queue of twenty dense layers stood still after eight,
-    // with no wait inside this kernel running out; a kernel of this length has nothing to gain from an early start anyway.
+    // An ordinary launch: a kernel of this length has little to gain from the early start of the short kernels' chains.
     mx_gemm_2cta_kernel<EPI><<<grid, kThreads, kSmem, stream>>>(p);
     return cudaGetLastError();
 }

@@ -526,3 +526,38 @@ def test_handles_of_two_streams_at_once():
     torch.cuda.synchronize()
     for (moe, _, Y), w in zip(runs, want):
         assert moe.device_status() == 0 and torch.equal(Y, w)
+
+
+def test_a_long_mixed_queue_on_three_streams():
+    """Thousands of products of every form, CTA pairs among them, dense on two streams and grouped on a third, without a wait in between."""
+    rng = np.random.default_rng(3)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    shapes = [(1, 2048, 1024), (2, 1024, 4096), (777, 520, 448), (4096, 2048, 2048), (9500, 1024, 64)]
+    layers = [[Layer(*f, 60 + i, s.cuda_stream) for i, f in enumerate(shapes)] for s in side]
+    want = [[l.run().clone() for l in ls] for ls in layers]
+    s = torch.cuda.Stream()
+    T, D, H, E, K = 6000, 256, 512, 16, 4
+    moe = M.MoE(T, D, E, K, hidden=H, training=False, stream=s.cuda_stream)
+    up, down = M.Mxfp4Weights(quantized(torch.randn(E, H, D).numpy() * 0.05)), M.Mxfp4Weights(quantized(torch.randn(E, D, H).numpy() * 0.05))
+    X, Wr, Y = bf((T, D), 1), bf((E, D), 2, 0.05), torch.zeros(T, D, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
+    y = Y.clone()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for _ in range(400):
+            i = rng.integers(0, 11)
+            if i == 10:
+                moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
+            else:
+                layers[i % 2][i // 2].run()
+        torch.cuda.synchronize()
+        assert moe.device_status() == 0 and torch.equal(Y, y)
+        for ls, ws in zip(layers, want):
+            for l, w in zip(ls, ws):
+                assert torch.equal(l.Y, w)
+                l.Y.zero_()
+        torch.cuda.synchronize()
+        for ls in layers:
+            for l in ls:
+                l.run()
