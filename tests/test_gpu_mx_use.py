@@ -36,6 +36,12 @@ class Layer:
         M.linear_mxfp4(self.X, self.W, self.Y, self.work, stream=self.stream)
         return self.Y
 
+    def value(self):
+        """A copy of what a call gives: the copy runs on another stream than the call, so it waits."""
+        self.run()
+        torch.cuda.synchronize()
+        return self.Y.clone()
+
 
 FORMS = [(5, 520, 320), (3, 264, 2112), (300, 264, 448), (9500, 512, 64)]          # few rows, few against a long k, some, many
 
@@ -193,7 +199,7 @@ def test_on_a_stream_of_its_own_an_operator_waits_for_that_stream(rows, n, k):
     layer = Layer(rows, n, k, 11, stream.cuda_stream)
     fresh = bf(layer.X.shape, 5)
     torch.cuda.synchronize()
-    want0 = layer.run().clone()
+    want0 = layer.value()
     with torch.cuda.stream(stream):
         torch.cuda._sleep(20_000_000)
         layer.X.copy_(fresh)
@@ -210,7 +216,7 @@ def test_on_a_stream_of_its_own_an_operator_waits_for_that_stream(rows, n, k):
 def test_two_streams_at_once():
     streams = [torch.cuda.Stream() for _ in range(2)]
     layers = [[Layer(*f, 20 + i, s.cuda_stream) for i, f in enumerate(FORMS)] for s in streams]
-    want = [[l.run().clone() for l in ls] for ls in layers]
+    want = [[l.value() for l in ls] for ls in layers]
     torch.cuda.synchronize()
     for ls in layers:
         for l in ls:
@@ -480,7 +486,7 @@ def test_every_form_recorded_side_by_side_and_replayed():
     """The layers fork onto two streams inside one recording and join again."""
     side = [torch.cuda.Stream() for _ in range(2)]
     layers = [Layer(*f, 40 + i, s.cuda_stream) for s in side for i, f in enumerate(FORMS)]
-    want = [l.run().clone() for l in layers]
+    want = [l.value() for l in layers]
     torch.cuda.synchronize()
     main, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     with torch.cuda.stream(main):
@@ -534,7 +540,7 @@ def test_a_long_mixed_queue_on_three_streams():
     side = [torch.cuda.Stream() for _ in range(2)]
     shapes = [(1, 2048, 1024), (2, 1024, 4096), (777, 520, 448), (4096, 2048, 2048), (9500, 1024, 64)]
     layers = [[Layer(*f, 60 + i, s.cuda_stream) for i, f in enumerate(shapes)] for s in side]
-    want = [[l.run().clone() for l in ls] for ls in layers]
+    want = [[l.value() for l in ls] for ls in layers]
     s = torch.cuda.Stream()
     T, D, H, E, K = 6000, 256, 512, 16, 4
     moe = M.MoE(T, D, E, K, hidden=H, training=False, stream=s.cuda_stream)
@@ -542,6 +548,7 @@ def test_a_long_mixed_queue_on_three_streams():
     X, Wr, Y = bf((T, D), 1), bf((E, D), 2, 0.05), torch.zeros(T, D, device="cuda").bfloat16()
     torch.cuda.synchronize()
     moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
+    torch.cuda.synchronize()
     y = Y.clone()
     torch.cuda.synchronize()
     for _ in range(10):
@@ -557,7 +564,9 @@ def test_a_long_mixed_queue_on_three_streams():
             for l, w in zip(ls, ws):
                 assert torch.equal(l.Y, w)
                 l.Y.zero_()
+        Y.zero_()
         torch.cuda.synchronize()
         for ls in layers:
             for l in ls:
                 l.run()
+        moe.forward_mxfp4(X, Wr, up, down, Y, 0.0)
