@@ -155,13 +155,15 @@ __global__ void __cluster_dims__(2, 1, 1) TMT_GEMM_BOUNDS gemm_tcgen05_2cta_kern
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    __syncwarp();
+    cluster_sync();            // the pair's allocation is one act of both CTAs: both are there, with their barriers, before it
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols2) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();            // both CTAs' barriers are initialised and both hold their TMEM
+    cluster_sync();            // both hold their TMEM
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
 
@@ -340,6 +342,8 @@ __global__ void __cluster_dims__(2, 1, 1) TMT_GEMM_BOUNDS gemm_tcgen05_2cta_kern
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols2) : "memory");
     }
+    __syncthreads();
+    cluster_sync();            // neither leaves before both have freed theirs (see mx_gemm_2cta.cu)
 }
 
 template <int EPI>
