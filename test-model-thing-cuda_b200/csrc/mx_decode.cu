@@ -401,7 +401,7 @@ cudaError_t launch_t(const MxDecode& p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int blocks = ((p.n + 127) / 128) * (p.experts ? p.experts : p.split);
     if constexpr (!SPLIT) return launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, stream, p, stages);
-    // a cluster per tile, launched the ordinary way (see mx_gemm_2cta.cu)
+    // a cluster per tile
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[1];
