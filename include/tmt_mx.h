@@ -74,7 +74,8 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
 /* tmt_moe_forward with both expert products on 4-bit blocks (hidden > 0, training = 0, a single rank). The router, the
  * gate weights, the statistics and the residual (beta) are those of tmt_moe_forward, bit for bit; a token's row is quantised
  * on its way into its experts' groups; P = q4(X) Wup^T, then q4(silu(P)) straight from the fp32 accumulators, then
- * gate * (q4(silu(P)) Wdown^T). Wup / Wdown: HOST arrays of E descriptors whose device memory must stay valid while the
+ * gate * (q4(silu(P)) Wdown^T): fp32, a token's rows and the residual added in fp32 and rounded once to bf16. (The bf16 block rounds every
+ * gated row before it adds; here a handle keeps them as fp32, 4 bytes for each of its grouped rows' elements.) Wup / Wdown: HOST arrays of E descriptors whose device memory must stay valid while the
  * handle uses them. The first call on a handle allocates its buffers, and a call with other pointers than the last one
  * uploads a table and waits for it: both are refused while the handle's stream is being captured. Other calls may be recorded;
  * a graph keeps the weights' addresses it was recorded with, whatever later calls are given. */

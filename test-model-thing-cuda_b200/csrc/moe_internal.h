@@ -31,9 +31,10 @@ struct Profiler {
     long long count[kNumPhases] = {0};
 };
 // Buffers of tmt_moe_forward_mxfp4 (mx_moe.cu), allocated at its first call: the grouped rows and their SiLU outputs as 4-bit
-// blocks, and the per-expert tables of the weights last handed in.
+// blocks, the gated outputs of the experts in fp32, and the per-expert tables of the weights last handed in.
 struct MxState {
     uint8_t *x_codes = nullptr, *x_scales = nullptr, *h_codes = nullptr, *h_scales = nullptr;
+    float* y_rows = nullptr;
     CUtensorMap x_map = {}, h_map = {}, x_sf = {}, h_sf = {}, y_out = {};
     CUtensorMap* tables = nullptr;                 // per-expert weight maps (mx_moe.cu)
     const uint8_t** scale_tab = nullptr;           // [2][E]

@@ -172,8 +172,8 @@ __device__ __forceinline__ void drain(const MxDecode& p, const uint16_t* list, i
                 q[i] |= __shfl_xor_sync(kFull, q[i], 1);
                 q[i] |= __shfl_xor_sync(kFull, q[i], 2);
                 q[i] |= __shfl_xor_sync(kFull, q[i], 4);
-            } else if constexpr (EPI == kMxF32) q[i] = __float_as_uint(x);
-            else q[i] = f2bf(EPI == kMxDown ? x * gate[i] : x);
+            } else if constexpr (EPI == kMxBf16) q[i] = f2bf(x);
+            else q[i] = __float_as_uint(EPI == kMxDown ? x * gate[i] : x);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -181,8 +181,8 @@ __device__ __forceinline__ void drain(const MxDecode& p, const uint16_t* list, i
             if constexpr (EPI == kMxUp) {
                 if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row[i] * p.n + col) / 2) = q[i];
                 if (lane == 0) p.out_scales[(size_t)row[i] * scale_tiles_k(p.n) * 4 + (col >> 5)] = (uint8_t)sb[i];
-            } else if constexpr (EPI == kMxF32) static_cast<float*>(p.out)[row[i] * p.n + col] = __uint_as_float(q[i]);
-            else static_cast<uint16_t*>(p.out)[row[i] * p.n + col] = (uint16_t)q[i];
+            } else if constexpr (EPI == kMxBf16) static_cast<uint16_t*>(p.out)[row[i] * p.n + col] = (uint16_t)q[i];
+            else static_cast<float*>(p.out)[row[i] * p.n + col] = __uint_as_float(q[i]);
         }
         __syncwarp();
     }

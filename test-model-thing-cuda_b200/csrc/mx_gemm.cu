@@ -97,7 +97,7 @@ __device__ __forceinline__ void drain_tile(const MxGemm& p, const Tile& ti, uint
         if (lane < rows)
             *reinterpret_cast<uint16_t*>(p.out_scales + scale_word(row, col0 >> 7, scale_tiles_k(p.n)) + ((col0 >> 5) & 3)) = (uint16_t)scales;
     } else {
-        constexpr int kBytes = EPI == kMxF32 ? 4 : 2, kBoxCols = 128 / kBytes;
+        constexpr int kBytes = EPI == kMxBf16 ? 2 : 4, kBoxCols = 128 / kBytes;
         uint8_t* out = static_cast<uint8_t*>(p.out);
 #pragma unroll
         for (int x0 = 0; x0 < 64; x0 += kBoxCols) {
@@ -107,7 +107,7 @@ __device__ __forceinline__ void drain_tile(const MxGemm& p, const Tile& ti, uint
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (EPI == kMxF32) w[i] = v[x0 + 4 * q + i];
-                    else if constexpr (EPI == kMxDown) w[i] = pack_pair(gate * __uint_as_float(v[8 * q + 2 * i]), gate * __uint_as_float(v[8 * q + 2 * i + 1]));
+                    else if constexpr (EPI == kMxDown) w[i] = __float_as_uint(gate * __uint_as_float(v[x0 + 4 * q + i]));
                     else w[i] = pack_pair(__uint_as_float(v[8 * q + 2 * i]), __uint_as_float(v[8 * q + 2 * i + 1]));
                 }
                 st_shared16(buf + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);

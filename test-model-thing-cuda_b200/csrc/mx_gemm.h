@@ -12,7 +12,7 @@ enum MxEpilogue : int {
     kMxBf16 = 0,     // out = bf16(acc), rows x n
     kMxF32 = 1,      // out = acc, rows x n
     kMxUp = 2,       // out = 4-bit codes of silu(acc), out_scales = their scale tiles
-    kMxDown = 3,     // out = bf16(row_scale[row] * acc)
+    kMxDown = 3,     // out = row_scale[row] * acc, fp32: a token's rows are added before anything is rounded
 };
 
 struct MxGemm {

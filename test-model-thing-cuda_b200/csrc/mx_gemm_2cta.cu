@@ -280,7 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
                     if (lane < rows)       // runs start on an even block
                         *reinterpret_cast<uint16_t*>(p.out_scales + scale_word(row, col0 >> 7, scale_tiles_k(p.n)) + ((col0 >> 5) & 3)) = (uint16_t)scales;
                 } else {
-                    constexpr int kBoxCols = EPI == kMxF32 ? 32 : 64;       // 128 bytes a row
+                    constexpr int kBoxCols = EPI == kMxBf16 ? 64 : 32;      // 128 bytes a row
 #pragma unroll
                     for (int x0 = 0; x0 < 64; x0 += kBoxCols) {
                         if (col0 + x0 >= p.n) continue;
@@ -292,7 +292,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 if constexpr (EPI == kMxF32) w[i] = v[x0 + 4 * q + i];
-                                else if constexpr (EPI == kMxDown) w[i] = pack_pair(gate * __uint_as_float(v[8 * q + 2 * i]), gate * __uint_as_float(v[8 * q + 2 * i + 1]));
+                                else if constexpr (EPI == kMxDown) w[i] = __float_as_uint(gate * __uint_as_float(v[x0 + 4 * q + i]));
                                 else w[i] = pack_pair(__uint_as_float(v[8 * q + 2 * i]), __uint_as_float(v[8 * q + 2 * i + 1]));
                             }
                             st_shared16(buf + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);

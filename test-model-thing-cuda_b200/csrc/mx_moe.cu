@@ -13,7 +13,6 @@
 #include "mx_decode.h"
 #include "mx_gemm.h"
 #include "mx_host.h"
-#include "nvfp4_decode.h"
 
 namespace tmt {
 namespace {
@@ -92,70 +91,73 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
     }
 }
 
-// Y[t] = beta * Y[t] + the token's K gated rows, added in fp32 in the order of its experts and rounded once: the sums of the bf16
-// block's combine, in its order. One warp per token; a lane has two vectors of every row in flight before it adds (with the row
-// count known to the compiler: in the bf16 block's kernel, which tests each row, 131072 tokens x 4 rows of 2048 took 509 us; here 396, 6.8 TB/s).
-template <int K>
-__global__ void __launch_bounds__(kDispatchWarps * 32) mx_combine_kernel(const RouteDims d, const RouteBufs b, const uint16_t* __restrict__ Yg,
+// Y[t] = beta * Y[t] + the token's K gated rows, fp32 rows added in fp32 in the order of its experts and rounded once. (Rows of bf16,
+// as the bf16 block keeps them, are half the bytes: at 131072 tokens x 4 of 2048 columns the product and this kernel took 925 + 400 us
+with them, and take 1150 + 728 now (6.6 TB/s); the output was off by 2.4e-3 of its norm, now by the 1.7e-3 of its own rounding.) A lane takes 4
+// columns and has two vectors of every row in flight before it adds, with the row count known to the compiler; a row of blocks
+// (blockIdx.y) takes every gridDim.y-th run of 256 columns, so that a few tokens spread over the SMs. DIRECT: the rows lie in the order of
+// the assignments (few-row products), else where the dispatch put them.
+template <int K, bool DIRECT>
+__global__ void __launch_bounds__(kDispatchWarps * 32) mx_combine_kernel(const RouteDims d, const RouteBufs b, const float* __restrict__ Yg,
                                                                          uint16_t* __restrict__ Y, float beta) {
     pdl_wait();
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const long t = (long)blockIdx.x * kDispatchWarps + (threadIdx.x >> 5);
     if (t >= d.T) return;
-    int slot = lane < K ? b.slot_of[t * K + lane] : 0;
-    const bool bad = slot < 0 || slot >= d.cap;               // a slot the dispatch refused: the row is left out
-    if (bad) { report(b.status, kErrSlotRange); slot = 0; }
-    const unsigned skip = __ballot_sync(0xffffffffu, bad);
-    const uint16_t* rows[K];
+    const float* rows[K];
+    unsigned skip = 0;
+    if constexpr (DIRECT) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) rows[j] = Yg + (long)__shfl_sync(0xffffffffu, slot, j) * d.D;
+        for (int j = 0; j < K; ++j) rows[j] = Yg + (t * K + j) * d.D;
+    } else {
+        int slot = lane < K ? b.slot_of[t * K + lane] : 0;
+        const bool bad = slot < 0 || slot >= d.cap;           // a slot the dispatch refused: the row is left out
+        if (bad) { report(b.status, kErrSlotRange); slot = 0; }
+        skip = __ballot_sync(0xffffffffu, bad);
+#pragma unroll
+        for (int j = 0; j < K; ++j) rows[j] = Yg + (long)__shfl_sync(0xffffffffu, slot, j) * d.D;
+    }
     uint16_t* dst = Y + t * d.D;
-    auto add = [&](int v, const uint4 (&x)[K], const uint4& y) {
-        float acc[8];
-        const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[2 * i] = beta != 0.0f ? beta * bf_lo(yw[i]) : 0.0f;
-            acc[2 * i + 1] = beta != 0.0f ? beta * bf_hi(yw[i]) : 0.0f;
-        }
+    auto add = [&](int v, const uint4 (&x)[K], const uint2& y) {
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (beta != 0.0f) { acc[0] = beta * bf_lo(y.x); acc[1] = beta * bf_hi(y.x); acc[2] = beta * bf_lo(y.y); acc[3] = beta * bf_hi(y.y); }
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            if (skip >> j & 1) continue;
-            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { acc[2 * i] += bf_lo(w[i]); acc[2 * i + 1] += bf_hi(w[i]); }
+            if (!DIRECT && (skip >> j & 1)) continue;
+            acc[0] += __uint_as_float(x[j].x); acc[1] += __uint_as_float(x[j].y);
+            acc[2] += __uint_as_float(x[j].z); acc[3] += __uint_as_float(x[j].w);
         }
-        uint4 o;
-        o.x = pack_bf2(acc[0], acc[1]); o.y = pack_bf2(acc[2], acc[3]); o.z = pack_bf2(acc[4], acc[5]); o.w = pack_bf2(acc[6], acc[7]);
-        stg16(dst + v, o);
+        *reinterpret_cast<uint2*>(dst + v) = make_uint2(pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3]));
     };
-    for (int v = lane * 8; v < d.D; v += 512) {
-        const bool two = v + 256 < d.D;
-        uint4 x0[K], x1[K], y0 = make_uint4(0, 0, 0, 0), y1 = y0;
+    for (int v = (int)blockIdx.y * 256 + lane * 4; v < d.D; v += 256 * (int)gridDim.y) {
+        const bool two = v + 128 < d.D;
+        uint4 x0[K], x1[K];
+        uint2 y0 = make_uint2(0, 0), y1 = y0;
 #pragma unroll
         for (int j = 0; j < K; ++j) x0[j] = ldg16_stream(rows[j] + v);
-        if (beta != 0.0f) y0 = ldg16(dst + v);
+        if (beta != 0.0f) y0 = *reinterpret_cast<const uint2*>(dst + v);
         if (two) {
 #pragma unroll
-            for (int j = 0; j < K; ++j) x1[j] = ldg16_stream(rows[j] + v + 256);
-            if (beta != 0.0f) y1 = ldg16(dst + v + 256);
+            for (int j = 0; j < K; ++j) x1[j] = ldg16_stream(rows[j] + v + 128);
+            if (beta != 0.0f) y1 = *reinterpret_cast<const uint2*>(dst + v + 128);
         }
         add(v, x0, y0);
-        if (two) add(v + 256, x1, y1);
+        if (two) add(v + 128, x1, y1);
     }
 }
-cudaError_t launch_mx_combine(const RouteDims& d, const RouteBufs& b, const uint16_t* Yg, uint16_t* Y, float beta, cudaStream_t s) {
-    const dim3 grid((d.T + kDispatchWarps - 1) / kDispatchWarps), block(kDispatchWarps * 32);
+template <bool DIRECT>
+cudaError_t launch_mx_combine(const RouteDims& d, const RouteBufs& b, const float* Yg, uint16_t* Y, float beta, cudaStream_t s) {
+    const dim3 grid((d.T + kDispatchWarps - 1) / kDispatchWarps, DIRECT ? (d.D + 255) / 256 : 1), block(kDispatchWarps * 32);
     switch (d.K) {
-        case 1: return launch_pdl(mx_combine_kernel<1>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 2: return launch_pdl(mx_combine_kernel<2>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 3: return launch_pdl(mx_combine_kernel<3>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 4: return launch_pdl(mx_combine_kernel<4>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 5: return launch_pdl(mx_combine_kernel<5>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 6: return launch_pdl(mx_combine_kernel<6>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 7: return launch_pdl(mx_combine_kernel<7>, grid, block, 0, s, d, b, Yg, Y, beta);
-        case 8: return launch_pdl(mx_combine_kernel<8>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 1: return launch_pdl(mx_combine_kernel<1, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 2: return launch_pdl(mx_combine_kernel<2, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 3: return launch_pdl(mx_combine_kernel<3, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 4: return launch_pdl(mx_combine_kernel<4, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 5: return launch_pdl(mx_combine_kernel<5, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 6: return launch_pdl(mx_combine_kernel<6, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 7: return launch_pdl(mx_combine_kernel<7, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
+        case 8: return launch_pdl(mx_combine_kernel<8, DIRECT>, grid, block, 0, s, d, b, Yg, Y, beta);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -190,7 +192,8 @@ void make_buffers(tmt_moe* h) {
     mx_make_map(&m.h_map, m.h_codes, cap, H, kMxBoxRows);
     mx_make_scale_map(&m.x_sf, m.x_scales, cap, D, kMxActBands);
     mx_make_scale_map(&m.h_sf, m.h_scales, cap, H, kMxActBands);
-    mx_make_out_map(&m.y_out, h->Yg, cap, D, false);
+    m.y_rows = alloc<float>(h, (size_t)cap * D);
+    mx_make_out_map(&m.y_out, m.y_rows, cap, D, true);
     // the padding rows' scale bytes are read with the others (their products are never used): give them a value
     cuda_ok(cudaMemsetAsync(m.x_scales, 0, scale_bytes(cap, D), h->stream), "cudaMemsetAsync");
     cuda_ok(cudaMemsetAsync(m.h_scales, 0, scale_bytes(cap, H), h->stream), "cudaMemsetAsync");
@@ -265,11 +268,11 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
         cuda_ok(launch_mx_decode(q, h->stream), "mx up launch");
         q.src = m.h_codes; q.src_scales = m.h_scales; q.src_kind = kMxSrcRows; q.src_mul = mx_row_factor(1);
         q.w_maps += (size_t)kTabsPerProduct * E; q.w_sf_maps += (size_t)kTabsPerProduct * E;
-        q.n = D; q.k = H; q.epi = kMxDown; q.out = h->Yg; q.out_scales = nullptr; q.gate = h->rb.w;
+        q.n = D; q.k = H; q.epi = kMxDown; q.out = m.y_rows; q.out_scales = nullptr; q.gate = h->rb.w;
         prof_mark(h, kPhGemmDown);
         cuda_ok(launch_mx_decode(q, h->stream), "mx down launch");
         prof_mark(h, kPhCombine);
-        cuda_ok(launch_decode_combine(h->Yg, static_cast<uint16_t*>(Y), beta, tokens, D, K, h->stream), "combine launch");
+        cuda_ok(launch_mx_combine<true>(h->dims, h->rb, m.y_rows, static_cast<uint16_t*>(Y), beta, h->stream), "combine launch");
         prof_mark(h, -1);
         h->launches += 3;
         h->have_forward = true;
@@ -295,14 +298,14 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     weights(0);
     prof_mark(h, kPhGemmUp);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
-    p.n = D; p.k = H; p.epi = kMxDown; p.out = h->Yg; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
+    p.n = D; p.k = H; p.epi = kMxDown; p.out = m.y_rows; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
     p.form = mx_form((long)tokens * K, E, p.n, p.k, h->num_sms, h->pad);
     p.act = m.h_map; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
     weights(1);
     prof_mark(h, kPhGemmDown);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx down launch");
     prof_mark(h, kPhCombine);
-    cuda_ok(launch_mx_combine(h->dims, h->rb, h->Yg, static_cast<uint16_t*>(Y), beta, h->stream), "combine launch");
+    cuda_ok(launch_mx_combine<false>(h->dims, h->rb, m.y_rows, static_cast<uint16_t*>(Y), beta, h->stream), "combine launch");
     prof_mark(h, -1);
     h->launches += 4;
     h->have_forward = true;

@@ -1,0 +1,75 @@
+"""What a value of the microscaled operators may depend on, and how exactly it is held: sums of a token's experts, tokens in any
+batch, normalised values of rows whose mean is far above their deviation."""
+import numpy as np
+import pytest
+import torch
+
+import mx_ref as R
+import tmt_moe_b200 as M
+from oracle import oracle as O
+from test_gpu_mx import FMT8, exact64, experts_case, ln_backward_ref, quantized, to_device
+
+pytestmark = pytest.mark.gpu
+
+
+def raw(n):
+    return torch.empty(n, dtype=torch.uint8, device="cuda")
+
+
+def bf(shape, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).bfloat16()
+
+
+def wide(shape, seed, scale=1.0):
+    """Blocks of many magnitudes: the sums of their products then take values all over, not a few thousand of a coarse grid."""
+    g = torch.Generator(device="cuda").manual_seed(seed + 1000)
+    e = torch.randint(-8, 1, (*shape[:-1], shape[-1] // 32), generator=g, device="cuda").repeat_interleave(32, -1)
+    return (bf(shape, seed, 2 * scale).float() * torch.exp2(e.float())).bfloat16()
+
+
+def wide_weights(E, n, k, seed):
+    return M.Mxfp4Weights(quantized(wide((E, n, k), seed, 0.1).float().cpu().numpy()))
+
+
+def bf64(w):
+    return O.bf16_to_f32(O.f32_to_bf16(np.asarray(w, np.float32))).astype(np.float64)
+
+
+def experts64(x, up, down, idx, w):
+    """float64 forward for the routing the handle chose, and the magnitudes that the fp32 sums of its down products run over."""
+    xq = R.q(x, "e2m1")
+    y, mag = np.zeros(x.shape), np.zeros(x.shape)
+    for e in range(len(up)):
+        t, j = np.where(idx == e)
+        if not len(t):
+            continue
+        p = xq[t] @ R.q(bf64(up[e]), "e2m1").T
+        h, dq, g = R.q(p / (1 + np.exp(-p)), "e2m1"), R.q(bf64(down[e]), "e2m1").T, w[t, j][:, None]
+        np.add.at(y, t, g * (h @ dq))
+        np.add.at(mag, t, g * (np.abs(h) @ np.abs(dq)))
+    return y, mag
+
+
+# few rows per expert, 128 x 128 tiles, CTA pairs (more than three turns of tiles)
+EXPERTS = [(40, 128, 128, 16, 4), (300, 128, 64, 12, 8), (300, 320, 192, 3, 3), (9000, 512, 512, 4, 2)]
+
+
+@pytest.mark.parametrize("beta", [0.0, -0.5])
+@pytest.mark.parametrize("T,D,H,E,K", EXPERTS)
+def test_the_experts_of_a_token_are_added_in_fp32(T, D, H, E, K, beta):
+    x, wr, up, down = experts_case(T, D, H, E, K, T + K)
+    moe = M.MoE(T, D, E, K, hidden=H, training=False)
+    y0 = bf((T, D), 3)
+    Y = y0.clone()
+    moe.forward_mxfp4(to_device(x, "bf16"), to_device(wr, "bf16"), quantized(up), quantized(down), Y, beta)
+    assert moe.device_status() == 0
+    y, mag = experts64(x, up, down, moe.read("idx"), moe.read("w").astype(np.float64))
+    want = y + beta * exact64(y0)
+    # one rounding to bf16 (half a step), and in front of it H products added in fp32, then the gate, K rows and the residual
+    tol = 2.0 ** -8 * np.abs(want) + (H + K + 4) * 2.0 ** -23 * (mag + np.abs(beta * exact64(y0)))
+    bad = (np.abs(exact64(Y) - want) > tol).any(1)
+    # An element of the hidden row that lies within fp32 error of the border between two codes may fall to the other side, which moves the
+    # whole token. That error is D 2^-23 of sum |x||w|, at most about 10^-4 of a block's scale, borders are half a scale apart, a token has
+    # H K elements: below 5 % of the tokens here, by the bound (far fewer in fact). Rows rounded to bf16 before they are added miss it everywhere.
+    assert bad.mean() <= 0.05, bad.mean()
