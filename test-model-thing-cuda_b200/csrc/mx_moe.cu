@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
 
 // Y[t] = beta * Y[t] + the token's K gated rows, fp32 rows added in fp32 in the order of its experts and rounded once. (Rows of bf16,
 // as the bf16 block keeps them, are half the bytes: at 131072 tokens x 4 of 2048 columns the product and this kernel took 925 + 400 us
-with them, and take 1150 + 728 now (6.6 TB/s); the output was off by 2.4e-3 of its norm, now by the 1.7e-3 of its own rounding.) A lane takes 4
+// with them, and take 1150 + 728 now (6.6 TB/s); the output was off by 2.4e-3 of its norm, now by the 1.7e-3 of its own rounding.) A lane takes 4
 // columns and has two vectors of every row in flight before it adds, with the row count known to the compiler; a row of blocks
 // (blockIdx.y) takes every gridDim.y-th run of 256 columns, so that a few tokens spread over the SMs. DIRECT: the rows lie in the order of
 // the assignments (few-row products), else where the dispatch put them.
