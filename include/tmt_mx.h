@@ -23,10 +23,8 @@
  * rows = 0 is allowed where no handle is involved and does nothing.
  *
  * Kernels of these operators may be scheduled while the one before them on the stream is still running (programmatic launch;
- * TMT_MOE_PDL=0 in the environment switches it off). They wait for it before they touch what it may write, with one exception:
- * products of few rows ask for their WEIGHTS at once. Weights written by tmt_moe_quantize_mxfp4, by copies, or by any kernel
- * that does not itself let its successor start early (no ordinary kernel does) are safe; a kernel of the caller's own that
- * calls griddepcontrol.launch_dependents before it has written a weight is not. */
+ * TMT_MOE_PDL=0 in the environment switches it off). They wait for it before they touch what it may write, weights among it: any tensor
+ * may be written by the call, copy or kernel right before the one that reads it. */
 #ifndef TMT_MX_H
 #define TMT_MX_H
 

@@ -2,7 +2,11 @@
 // microseconds each): a kernel launched with the attribute may be scheduled, and run whatever precedes its
 // `pdl_wait()`, while the kernel before it in the stream is still running; `pdl_wait()` returns once that kernel
 // has completed and its writes are visible. Every kernel of such a chain calls `pdl_begin()` first (lets its own
-// successor be scheduled early) and touches nothing another kernel reads or writes before `pdl_wait()`. Without the
+// successor be scheduled early) and touches nothing another kernel reads or writes before `pdl_wait()`. The one thing read
+// before it are the expert weights of the decode steps (nvfp4_decode.cu, mx_decode.cu): no kernel of the chain writes them, and the chain's first
+// kernel (router_logits_small_kernel, or an ordinary launch) waits for all that came before the chain before it lets the second
+// start. That kernel's end alone would not do: a successor may start when its predecessor's blocks have ended, but the
+// predecessor's writes are promised to be visible only after `pdl_wait()`. Without the
 // attribute both calls do nothing. TMT_MOE_PDL=0 launches the chain the ordinary way.
 #pragma once
 #include <cuda_runtime.h>

@@ -5,7 +5,7 @@
 // byte moves once; bound by HBM. In 4 bits a warp takes the same 256 columns of the rows r, r + 32, r + 64 and r + 96 of a band of 128,
 // whose scale words are neighbours in the scale tile (single words, one row a warp, took 150 us instead of 114 at 131072 x 2048). Several such chunks are in flight per warp where there are enough of them (U).
 // `early`: lets the next kernel of the stream be scheduled at once (launch_pdl.cuh). Only where that kernel is known to wait
-// before it reads what this one writes: the product of a dense layer, which starts on its weights without waiting.
+// before it reads anything: the product of a dense layer, whose barriers and tensor memory are then ready when this kernel ends.
 #include <cuda_runtime.h>
 
 #include "../../include/tmt_mx.h"

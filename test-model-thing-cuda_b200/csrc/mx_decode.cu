@@ -2,8 +2,11 @@
 // short kernels.
 //
 // A block (with a long k and few matrices: a cluster, each block a share of k) owns 128 weight rows of one matrix, the 128-row side of the MMA; the matrix's activation rows are its columns, 32 at a
-// time. At its start, before it knows whether and by whom the matrix is used, it asks for all of its weights (up to the shared
-// memory there is: 64 bytes per row and 128 of k), so that every weight of the product is on its way at once. Meanwhile sixteen
+// time. It asks for all of its weights (up to the shared memory there is: 64 bytes per row and 128 of k) before it knows whether and by whom
+// the matrix is used, so that every weight of the product is on its way at once: in the experts' chain at its start, while the kernel before it
+// is still running (the chain's first kernel has waited for whoever wrote them); a dense layer's only after it has waited, since the kernel
+// before it may be the one that writes them, and writes are promised to be visible after griddepcontrol.wait alone (1 row, 1024 -> 2048, in a
+// queue of such layers: 4.6 us; 4.3 when it did not wait, which read weights that might still be on their way). Meanwhile sixteen
 // warps find the matrix's rows in the router's index table (grouped) and bring them in: as values, which they quantise here, or
 // as codes. There is no separate quantising or dispatching kernel, and no row moves through memory twice.
 // Activations stay in shared memory for the whole of k in the order the MMA reads them (128-byte swizzle, scale tiles).
@@ -234,8 +237,11 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
         tma_load_2d(codes_w + s * kCodesW, map, fb, (kb0 + kb) * 128, w0);
         tma_load_3d(sf_w + s * kSfW, sf_map, fb, 0, 2 * (kb0 + kb), w0 >> 7);
     };
-    // Weights depend on no earlier kernel of the step. With fewer assignments than experts most blocks would ask in vain: they wait.
+    // With fewer assignments than experts most blocks would ask in vain: they look first.
     const bool ahead = p.experts == 0 || p.n_asg >= p.experts;
+    auto load_first = [&](int& issued) {
+        for (; issued < min(stages, nkb); ++issued) load_stage(issued, issued);
+    };
     int issued = 0;                          // loads so far (lane 0 of the TMA warp)
     if (warp == kTmaWarp && lane == 0) {
         abort_s = 0;
@@ -245,8 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (p.w_maps) { tensormap_acquire(map); tensormap_acquire(sf_map); }
-        if (ahead)
-            for (; issued < min(stages, nkb); ++issued) load_stage(issued, issued);
+        if (ahead && p.weights_ready) load_first(issued);
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
@@ -255,6 +260,8 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     }
     __syncwarp();
     pdl_wait();
+    if (warp == kTmaWarp && lane == 0 && ahead) load_first(issued);
+    __syncwarp();
     const int count = p.experts ? make_list(p, e, list, lane) : p.rows;
     const int passes = (count + kRows - 1) / kRows;
     tc_fence_before();

@@ -28,6 +28,7 @@ struct MxDecode {
     const float* gate;                 // kMxDown: per assignment
     int* status;
     bool early;                        // the next kernel waits by itself: it may be scheduled at once
+    bool weights_ready;                // a kernel between the weights' writer and this one has waited for it (griddepcontrol.wait), or this one's launch does
 };
 
 // a * factor >> 16 == a / divisor for a < 2048, divisor <= 8: the excess a * (factor - 65536 / divisor) / 65536 is below a / 65536 < 1 / 8.

@@ -261,6 +261,7 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
         MxDecode q;
         memset(&q, 0, sizeof q);
         q.idx = h->rb.idx; q.n_asg = tokens * K; q.experts = E; q.status = h->rb.status; q.early = true; q.split = 1;
+        q.weights_ready = true;              // the router's first kernel waits before it lets the next one start
         q.src = X; q.src_kind = kMxSrcBf16; q.src_mul = mx_row_factor(K);
         q.w_maps = m.tables + (size_t)kTabCodes * E; q.w_sf_maps = m.tables + (size_t)kTabScales1 * E;
         q.n = H; q.k = D; q.epi = kMxUp; q.out = m.h_codes; q.out_scales = m.h_scales;
@@ -326,6 +327,7 @@ void few_rows(const void* src, const void* scales, int kind, int rows, const tmt
     p.src = src; p.src_scales = static_cast<const uint8_t*>(scales); p.src_kind = kind;
     p.rows = rows; p.n = W.rows; p.k = W.cols;
     p.split = mx_decode_split(W.rows, W.cols, sm_count());
+    p.weights_ready = p.split > 1;           // clusters are launched the ordinary way, after all that came before
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
     cuda_ok(launch_mx_decode(p, s), "matmul_mxfp4 launch");
 }
