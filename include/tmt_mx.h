@@ -58,8 +58,8 @@ int tmt_moe_dequantize_mxfp4(const void* codes, const void* scales, long long ro
 
 /* Y = A W^T with both operands in 4-bit blocks, on the block-scaled tensor-core instruction: products exact, sums in fp32,
  * rounded once to `dtype`. A (rows, W->cols), Y (rows, W->rows) row-major and dense; W->rows: a multiple of 8, W->cols: a
- * multiple of 64. status (device int, may be NULL): receives a code of tmt_moe_device_status when a bounded wait ran out;
- * never cleared here. */
+ * multiple of 64. How k is shared among blocks depends on `rows`, and with it the last bits of a sum. status (device int, may
+ * be NULL): receives a code of tmt_moe_device_status when a bounded wait ran out; never cleared here. */
 int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, const tmt_mxfp4_weight* W, void* Y, int dtype,
                          int* status, void* stream);
 
@@ -69,14 +69,16 @@ size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols);
 int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
                          size_t work_bytes, int* status, void* stream);
 
-/* tmt_moe_forward with both expert products on 4-bit blocks (hidden > 0, training = 0, a single rank). The router, the
- * gate weights, the statistics and the residual (beta) are those of tmt_moe_forward, bit for bit; a token's row is quantised
- * on its way into its experts' groups; P = q4(X) Wup^T, then q4(silu(P)) straight from the fp32 accumulators, then
- * gate * (q4(silu(P)) Wdown^T): fp32, a token's rows and the residual added in fp32 and rounded once to bf16. (The bf16 block rounds every
- * gated row before it adds; here a handle keeps them as fp32, 4 bytes for each of its grouped rows' elements.) Wup / Wdown: HOST arrays of E descriptors whose device memory must stay valid while the
- * handle uses them. The first call on a handle allocates its buffers, and a call with other pointers than the last one
- * uploads a table and waits for it: both are refused while the handle's stream is being captured. Other calls may be recorded;
- * a graph keeps the weights' addresses it was recorded with, whatever later calls are given. */
+/* tmt_moe_forward with both expert products on 4-bit blocks (hidden > 0, training = 0, a single rank). The router, the gate
+ * weights, the statistics and the residual (beta) are those of tmt_moe_forward, bit for bit; a token's row is quantised on its
+ * way into its experts' groups; P = q4(X) Wup^T, then q4(silu(P)) straight from the fp32 accumulators, then gate *
+ * (q4(silu(P)) Wdown^T): fp32, a token's rows and the residual added in fp32 and rounded once to bf16. (The bf16 block rounds
+ * every gated row before it adds; here a handle keeps them as fp32, 4 bytes for each of its grouped rows' elements.) A token's
+ * output depends on its own row alone, bit for bit: not on its neighbours, nor on how many tokens a call has. Wup / Wdown:
+ * HOST arrays of E descriptors whose device memory must stay valid while the handle uses them. The first call on a handle
+ * allocates its buffers, and a call with other pointers than the last one uploads a table and waits for it: both are refused
+ * while the handle's stream is being captured. Other calls may be recorded; a graph keeps the weights' addresses it was
+ * recorded with, whatever later calls are given. */
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
                           const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
 

@@ -168,7 +168,7 @@ __device__ __forceinline__ void drain(const MxDecode& p, const uint16_t* list, i
         for (int i = 0; i < 4; ++i) {
             const float x = __uint_as_float(v[i]);
             if constexpr (EPI == kMxUp) {        // the warp's 32 outputs are one block
-                const float s = x * sigmoid_fast(x);
+                const float s = silu_lane(x);
                 sb[i] = scale_byte<kE2M1>(__reduce_max_sync(kFull, __float_as_uint(s) & 0x7fffffffu));
                 const float f[8] = {s * inv_scale(sb[i]), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
                 q[i] = sb[i] == 255u ? 0u : (pack_e2m1x8(f) & 15u) << (4 * (lane & 7));

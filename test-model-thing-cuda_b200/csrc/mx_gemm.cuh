@@ -106,15 +106,18 @@ __device__ __forceinline__ void tmem_wait64(uint32_t (&r)[64]) {
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float rcp_fast(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// silu of 32 accumulators, in place. The special-function unit sets the pace of this epilogue (16 results a clock and SM): two
-// elements share one reciprocal, 1 / a = b / (a b), so that an element costs 1.5 of its results instead of 2. a b stays finite,
-// and its reciprocal a normal number, while both exponents are below 43; a warp that holds an element below -43 takes the plain form.
+// silu of a block of 32 accumulators, in place. The special-function unit sets the pace of this epilogue (16 results a clock and SM): two
+// neighbours share one reciprocal, 1 / a = b / (a b), so that an element costs 1.5 of its results instead of 2. a b stays finite,
+// and its reciprocal a normal number, while both exponents are below 43; a block that holds an element below -43 takes the plain form.
+// The choice is the block's own (a thread holds it whole), never the warp's, whose other lanes are other tokens; silu_lane is the same
+// function with a block in the lanes of a warp, bit for bit. So a token's hidden row is the same in any batch.
+constexpr float kMinusLog2e = -1.4426950408889634f, kSiluPairMin = -43.0f;
 __device__ __forceinline__ void silu32(float (&f)[32]) {
     float lo = fminf(f[0], f[1]);
 #pragma unroll
     for (int i = 2; i < 32; i += 2) lo = fminf(fminf(lo, f[i]), f[i + 1]);
-    if (__all_sync(0xffffffffu, lo > -43.0f)) {          // false for a NaN in every element alone; others propagate through either form
-        const float2 c = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.0f, 1.0f);
+    if (lo > kSiluPairMin) {                             // false for a NaN in every element alone; others propagate through either form
+        const float2 c = make_float2(kMinusLog2e, kMinusLog2e), one = make_float2(1.0f, 1.0f);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
             const float2 x = make_float2(f[i], f[i + 1]);
@@ -128,6 +131,11 @@ __device__ __forceinline__ void silu32(float (&f)[32]) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = f[i] * sigmoid_fast(f[i]);
     }
+}
+__device__ __forceinline__ float silu_lane(float x) {
+    const float e = __fadd_rn(exp2_fast(__fmul_rn(x, kMinusLog2e)), 1.0f), other = __shfl_xor_sync(0xffffffffu, e, 1);
+    const float r = rcp_fast(__fmul_rn(e, other));
+    return __any_sync(0xffffffffu, x <= kSiluPairMin) ? x * sigmoid_fast(x) : __fmul_rn(x, __fmul_rn(r, other));
 }
 // One block of 32 -> its 4-bit codes, element 0 in the lowest nibble of q[0]; returns the scale byte.
 __device__ __forceinline__ uint32_t quantize32(const float (&f)[32], uint32_t (&q)[4]) {

@@ -73,3 +73,35 @@ def test_the_experts_of_a_token_are_added_in_fp32(T, D, H, E, K, beta):
     # whole token. That error is D 2^-23 of sum |x||w|, at most about 10^-4 of a block's scale, borders are half a scale apart, a token has
     # H K elements: below 5 % of the tokens here, by the bound (far fewer in fact). Rows rounded to bf16 before they are added miss it everywhere.
     assert bad.mean() <= 0.05, bad.mean()
+
+
+def test_a_token_does_not_depend_on_the_values_of_its_neighbours():
+    """Every sixteenth token has pre-activations far below zero: the others keep their bits."""
+    T, D, H, E, K = 65536, 256, 4096, 16, 2                          # 5 10^8 hidden elements: a last bit moves one in 10^7 to another code
+    up, down = wide_weights(E, H, D, 1), wide_weights(E, D, H, 2)
+    X, Wr, Y = wide((T, D), 3, 2.0), bf((E, D), 4, 0.05), torch.zeros(T, D, device="cuda").bfloat16()
+    keep = torch.arange(T, device="cuda") % 16 != 5
+    for tokens in (T, 300, 40):                                      # CTA pairs, tiles, few rows
+        moe = M.MoE(T, D, E, K, hidden=H, training=False)
+        moe.forward_mxfp4(X, Wr, up, down, Y, 0.0, tokens=tokens)
+        want = Y.clone()
+        big = torch.where(keep[:, None], X, X * 2048)                # the same experts: logits scaled by a power of two
+        moe.forward_mxfp4(big, Wr, up, down, Y, 0.0, tokens=tokens)
+        assert moe.device_status() == 0
+        n = keep[:tokens]
+        assert torch.equal(Y[:tokens][n], want[:tokens][n]) and not torch.equal(Y[:tokens], want[:tokens])
+
+
+def test_a_token_does_not_depend_on_the_size_of_its_batch():
+    """CTA pairs for the whole batch, 128 x 128 tiles and the few-row kernel for parts of it: the same bits."""
+    T, D, H, E, K = 24000, 128, 4096, 16, 2
+    up, down = wide_weights(E, H, D, 1), wide_weights(E, D, H, 2)
+    X, Wr, want = wide((T, D), 3, 2.0), bf((E, D), 4, 0.05), torch.zeros(T, D, device="cuda").bfloat16()
+    moe = M.MoE(T, D, E, K, hidden=H, training=False)
+    moe.forward_mxfp4(X, Wr, up, down, want, 0.0)
+    for step, n in ((300, T), (40, T), (1, 200)):
+        Y = torch.zeros_like(want)
+        for t in range(0, n, step):
+            moe.forward_mxfp4(X[t:t + step], Wr, up, down, Y[t:t + step], 0.0, tokens=step)
+        assert moe.device_status() == 0
+        assert torch.equal(Y[:n], want[:n]), step
