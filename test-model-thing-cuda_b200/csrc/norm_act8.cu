@@ -3,7 +3,9 @@
 //   xh = (x - mean) * rstd,  g = dy * gamma,  a = sum(g) / D,  b = sum(g * xh) / D
 //   dx = rstd * (g - a - xh * b),   dGamma[d] = sum over rows of dy * xh,   dBeta[d] = sum over rows of dy
 //
-// x is never written out: an element enters as its code, and xh = fma(code, scale * rstd, -mean * rstd).
+// x is never written out: an element enters as its code, and xh = fma(code, scale, -mean) * rstd: code * scale is exact, so x - mean is
+// rounded once, and a row whose mean is far above its deviation keeps its bits (fma(code, scale * rstd, -mean * rstd) would leave the
+// rounding of mean * rstd in a constant row).
 // A team walks a contiguous range of rows; a thread owns one vector of 8 columns (16 bytes of dY, 8 bytes of codes) of every row
 // (V = 2 vectors, half a row apart, where dim > 2048), so gamma and the column sums stay in its registers. A team is a block of
 // ceil(dim / 256) warps; for dim < 256 it is the smallest power of two of lanes that covers a row. RI rows are reduced together:
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_act8_kernel(const uint8_t* 
         for (int j = 0; j < RI; ++j) {
             const Raw<V> w = nxt[j];
             rs[j] = w.rstd;
-            const float2 c = bc(-w.mean * w.rstd);
+            const float2 minus_mean = bc(-w.mean), r2 = bc(w.rstd);
             float2 s1 = bc(0.0f), s2 = bc(0.0f);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
@@ -171,12 +173,12 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_act8_kernel(const uint8_t* 
                     const uint32_t at = (slot0 + j) * slot_bytes + k * vec_bytes;
                     dy4 = lds16(ring_dy + at); x8 = lds8(ring_x + at);
                 }
-                const float2 sc = bc(scale_value(w.sb[k]) * w.rstd);
+                const float2 sc = bc(scale_value(w.sb[k]));
                 const uint32_t dw[4] = {dy4.x, dy4.y, dy4.z, dy4.w}, xw[2] = {x8.x, x8.y};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 dy = make_float2(bf_lo(dw[i]), bf_hi(dw[i]));
-                    xh[j][k][i] = __ffma2_rn(unpack_f8x2<FMT>((uint16_t)(xw[i >> 1] >> (16 * (i & 1)))), sc, c);
+                    xh[j][k][i] = __fmul2_rn(__ffma2_rn(unpack_f8x2<FMT>((uint16_t)(xw[i >> 1] >> (16 * (i & 1)))), sc, minus_mean), r2);
                     g[j][k][i] = __fmul2_rn(dy, gam[k][i]);
                     s1 = __fadd2_rn(s1, g[j][k][i]);
                     s2 = __ffma2_rn(g[j][k][i], xh[j][k][i], s2);

@@ -105,3 +105,49 @@ def test_a_token_does_not_depend_on_the_size_of_its_batch():
             moe.forward_mxfp4(X[t:t + step], Wr, up, down, Y[t:t + step], 0.0, tokens=step)
         assert moe.device_status() == 0
         assert torch.equal(Y[:n], want[:n]), step
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("rows,dim", [(5, 32), (37, 96), (130, 256), (64, 1280), (9, 4096)])
+def test_a_constant_row_has_normalised_values_of_zero(rows, dim, fmt):
+    """x - mean is zero, whatever x is: no rounding of mean * rstd may be left over."""
+    c = np.resize([1.75, -7.0, 448.0, 1.5 * 2.0 ** 11, 1.25 * 2.0 ** -9, -1.75 * 2.0 ** 20], rows)
+    X, dY = to_device(np.repeat(c[:, None], dim, 1), "bf16"), bf((rows, dim), 5)
+    gamma, beta = bf((dim,), 6).float(), bf((dim,), 7).float()
+    Y, dX = torch.empty_like(X), torch.empty_like(X)
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    codes, scales, scratch = raw(rows * dim), raw(rows * dim // 32), raw(M.ln_backward_act8_scratch_bytes(rows, dim))
+    M.ln_forward_act8(X, gamma, beta, Y, mean, rstd, codes, scales, FMT8[fmt])
+    np.testing.assert_array_equal(exact64(mean), c)                  # sums of at most 4096 equal values of a few bits: exact
+    rstd.fill_(300.1)                                                # as if eps were a little larger: a number of 24 bits
+    top = exact64(rstd)[0]
+    dg, db = torch.full((dim,), 7.0, device="cuda"), torch.empty(dim, device="cuda")
+    M.ln_backward_act8(codes, scales, dY, gamma, mean, rstd, dX, dg, db, scratch, FMT8[fmt])
+    assert (dg == 0).all()
+    g = exact64(dY) * exact64(gamma)
+    want = top * (g - g.mean(1, keepdims=True))
+    # half a step of bf16; a sum of dim terms in fp32, and three more roundings
+    tol = 2.0 ** -8 * np.abs(want) + top * 2.0 ** -24 * ((dim + 4) * np.abs(g).mean(1, keepdims=True) + 4 * np.abs(g))
+    assert (np.abs(exact64(dX) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("rows,dim", [(37, 96), (300, 512), (21, 2080)])
+def test_layernorm_gradient_of_rows_far_from_zero(rows, dim, fmt):
+    """A mean some thousand deviations away: the normalised value keeps the bits that x - mean has."""
+    rng = np.random.default_rng(rows)
+    x = np.repeat(np.resize([3072.0, -1792.0, 0.4375], rows)[:, None], dim, 1)          # what the checkpoint holds of such a row
+    m64 = to_device(x[:, 0] * (1 + 2.0 ** -11 * rng.standard_normal(rows)), "f32")
+    codes, scales = (torch.from_numpy(a).cuda().reshape(-1) for a in R.quantize(x, fmt))
+    rstd = to_device(np.abs(3.0 / (x[:, 0] - exact64(m64))) * 0.3, "f32")              # xh of about 1: the statistics are an input
+    dY, gamma = bf((rows, dim), 8), bf((dim,), 9).float()
+    dX, dg, db = torch.empty(rows, dim, device="cuda").bfloat16(), torch.empty(dim, device="cuda"), torch.empty(dim, device="cuda")
+    M.ln_backward_act8(codes, scales, dY, gamma, m64, rstd, dX, dg, db, raw(M.ln_backward_act8_scratch_bytes(rows, dim)), FMT8[fmt])
+    dy = exact64(dY)
+    dx, wg, wb, xh, g = ln_backward_ref(x, dy, exact64(gamma), exact64(m64), exact64(rstd))
+    u = 2.0 ** -24
+    # x - mean and its product with rstd: two roundings of xh itself; column sums of `rows` terms
+    assert (np.abs(exact64(dg) - wg) <= (rows + 4) * u * np.abs(dy * xh).sum(0)).all()
+    s = np.abs(g * xh).sum(1, keepdims=True) / dim
+    tol = 2.0 ** -8 * np.abs(dx) + (dim + 8) * u * exact64(rstd)[:, None] * (np.abs(g) + np.abs(g).mean(1, keepdims=True) + np.abs(xh) * s)
+    assert (np.abs(exact64(dX) - dx) <= tol).all()
