@@ -331,7 +331,7 @@ __global__ void ln_bwd_reduce_kernel(const float* __restrict__ part, int blocks,
     if (i < D) dGamma[i] = s; else dBeta[i - D] = s;
 }
 
-int bwd_blocks(int rows) { return (rows + kBwdRows - 1) / kBwdRows; }
+int bwd_blocks(int rows) { return (rows - 1) / kBwdRows + 1; }
 
 void check_shape(int rows, int dim, int max_dim) {
     if (rows < 1 || dim < 8 || dim % 8 || dim > max_dim)
@@ -345,7 +345,7 @@ void launch_ln_fwd(const void* X, const float* gamma, const float* beta, void* Y
     int dev = 0, sms = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int want = (rows + kFwdWarps - 1) / kFwdWarps;
+    const int want = (rows - 1) / kFwdWarps + 1;
     const dim3 grid(std::max(1, std::min(want, std::max(sms, 1) * 6))), block(kFwdWarps * 32);      // a multiple of the SM count
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint16_t* x = static_cast<const uint16_t*>(X);

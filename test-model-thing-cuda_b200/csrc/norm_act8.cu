@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_act8_kernel(const uint8_t* 
         }
     }
     const float inv_d = 1.0f / (float)D;
-    const int rpt = (rows + teams - 1) / teams;      // rows of a team
+    const int rpt = (rows - 1) / teams + 1;          // rows of a team
     const long first = (long)team * rpt;
     const int n = (int)max(0L, min((long)rpt, rows - first));
     const uint32_t vec_bytes = blockDim.x * 24, slot_bytes = V * vec_bytes;
@@ -270,7 +270,7 @@ Plan plan(int rows, int dim) {
     p.threads = p.lanes < 32 ? 128 : threads;
     const int per_block = p.lanes < 32 ? p.threads / p.lanes : 1;
     const int resident = std::max(1, std::min(24, 512 / p.threads)) * kSms;      // 16 warps an SM hold 128 registers each
-    const int want = (rows + kMinRows * per_block - 1) / (kMinRows * per_block);
+    const int want = (rows - 1) / (kMinRows * per_block) + 1;
     p.blocks = std::max(1, std::min(want, resident));
     p.teams = p.blocks * per_block;
     return p;
