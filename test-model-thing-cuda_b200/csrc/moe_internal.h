@@ -10,7 +10,7 @@
 
 #include "../../include/tmt_moe.h"
 #include "kernels.cuh"
-#include "mx_gemm.h"
+#include "mx_state.h"
 
 struct tmt_ep_state;
 
@@ -29,17 +29,6 @@ struct Profiler {
     std::vector<std::pair<int, size_t>> marks;   // (phase or -1 = end of step, event index)
     double ms[kNumPhases] = {0};
     long long count[kNumPhases] = {0};
-};
-// Buffers of tmt_moe_forward_mxfp4 (mx_moe.cu), allocated at its first call: the grouped rows and their SiLU outputs as 4-bit
-// blocks, the gated outputs of the experts in fp32, and the per-expert tables of the weights last handed in.
-struct MxState {
-    uint8_t *x_codes = nullptr, *x_scales = nullptr, *h_codes = nullptr, *h_scales = nullptr;
-    float* y_rows = nullptr;
-    CUtensorMap x_map = {}, h_map = {}, x_sf = {}, h_sf = {}, y_out = {};
-    CUtensorMap* tables = nullptr;                 // per-expert weight maps (mx_moe.cu)
-    const uint8_t** scale_tab = nullptr;           // [2][E]
-    std::vector<const void*> key;                  // the pointers the tables were built from
-    bool recorded = false;                         // a graph was recorded with these tables
 };
 }  // namespace tmt
 

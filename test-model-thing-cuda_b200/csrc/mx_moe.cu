@@ -4,6 +4,7 @@
 // weight) and the combine below. With few rows per expert (mx_decode.cu) there is no dispatch.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/tmt_mx.h"
 #include "launch_pdl.cuh"
@@ -165,39 +166,34 @@ cudaError_t launch_mx_combine(const RouteDims& d, const RouteBufs& b, const floa
 // Per-expert maps: of each product the codes, and the scale tiles in boxes of one band (decode form) and of two (pair form).
 enum Table : int { kTabCodes = 0, kTabScales1, kTabScales2, kTabsPerProduct, kTables = 2 * kTabsPerProduct };
 
-template <class T>
-T* alloc(tmt_moe* h, size_t n) {
+void* alloc(tmt_moe* h, size_t bytes) {
     void* p = nullptr;
-    cuda_ok(cudaMalloc(&p, n * sizeof(T)), "cudaMalloc");
+    cuda_ok(cudaMalloc(&p, bytes), "cudaMalloc");
     h->allocs.push_back(p);
-    h->bytes += n * sizeof(T);
-    return static_cast<T*>(p);
-}
-
-void new_tables(tmt_moe* h) {
-    h->mx.tables = alloc<CUtensorMap>(h, kTables * (size_t)h->d.experts);
-    h->mx.scale_tab = alloc<const uint8_t*>(h, 2 * (size_t)h->d.experts);
-    h->mx.recorded = false;
+    h->bytes += bytes;
+    return p;
 }
 
 void make_buffers(tmt_moe* h) {
     MxState& m = h->mx;
-    const int D = h->d.dim, H = h->d.hidden, E = h->d.experts;
+    const int D = h->d.dim, H = h->d.hidden;
     const long cap = h->dims.cap;
-    m.x_codes = alloc<uint8_t>(h, (size_t)cap * D / 2);
-    m.x_scales = alloc<uint8_t>(h, scale_bytes(cap, D));
-    m.h_codes = alloc<uint8_t>(h, (size_t)cap * H / 2);
-    m.h_scales = alloc<uint8_t>(h, scale_bytes(cap, H));
+    // what an earlier call got before memory ran out is kept
+    auto need = [&](auto*& p, size_t n) { if (!p) p = static_cast<std::remove_reference_t<decltype(p)>>(alloc(h, n * sizeof *p)); };
+    need(m.x_codes, (size_t)cap * D / 2);
+    need(m.x_scales, scale_bytes(cap, D));
+    need(m.h_codes, (size_t)cap * H / 2);
+    need(m.h_scales, scale_bytes(cap, H));
+    need(m.y_rows, (size_t)cap * D);
     mx_make_map(&m.x_map, m.x_codes, cap, D, kMxBoxRows);
     mx_make_map(&m.h_map, m.h_codes, cap, H, kMxBoxRows);
     mx_make_scale_map(&m.x_sf, m.x_scales, cap, D, kMxActBands);
     mx_make_scale_map(&m.h_sf, m.h_scales, cap, H, kMxActBands);
-    m.y_rows = alloc<float>(h, (size_t)cap * D);
     mx_make_out_map(&m.y_out, m.y_rows, cap, D, true);
     // the padding rows' scale bytes are read with the others (their products are never used): give them a value
     cuda_ok(cudaMemsetAsync(m.x_scales, 0, scale_bytes(cap, D), h->stream), "cudaMemsetAsync");
     cuda_ok(cudaMemsetAsync(m.h_scales, 0, scale_bytes(cap, H), h->stream), "cudaMemsetAsync");
-    new_tables(h);
+    m.buffers = true;
 }
 
 bool capturing(cudaStream_t s) {
@@ -215,15 +211,14 @@ void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_wei
     std::vector<const void*> key(4 * (size_t)E);
     for (int e = 0; e < E; ++e) { key[e] = Wup[e].scales; key[E + e] = Wdown[e].scales; key[2 * E + e] = Wup[e].codes; key[3 * E + e] = Wdown[e].codes; }
     const bool recording = capturing(h->stream);
-    if (m.tables && key == m.key) {
+    if (key == m.key) {
         m.recorded |= recording;
         return;
     }
     if (recording)
         throw std::runtime_error("forward_mxfp4: the first call on a handle, and the first one with other weights, cannot be recorded into a graph; make one outside the capture");
-    if (!m.tables) make_buffers(h);
-    if (m.recorded) new_tables(h);
-    m.key.clear();                       // stays empty if anything below throws
+    if (!m.buffers) make_buffers(h);
+    m.open_tables(kTables * (size_t)E, 2 * (size_t)E, [&](size_t bytes) { return alloc(h, bytes); });
     for (const void* p : key) check_tensors({p});
     std::vector<CUtensorMap> maps(kTables * (size_t)E);
     for (int product = 0; product < 2; ++product)
