@@ -81,6 +81,9 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
  * recorded with, whatever later calls are given. */
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
                           const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
+/* 1 when the weights last handed to tmt_moe_forward_mxfp4 were recorded into a graph (which goes on reading them), else 0; -1 for a
+ * null handle. */
+int tmt_moe_mxfp4_recorded(const tmt_moe* h);
 
 /* 8-bit checkpoint of an activation X (rows, cols), and back. format: TMT_ACT8_E4M3 or TMT_ACT8_E5M2; cols: a multiple of 32. */
 int tmt_moe_act8_save(const void* X, int dtype, long long rows, int cols, int format, void* codes, void* scales, void* stream);

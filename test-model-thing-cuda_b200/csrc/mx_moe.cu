@@ -406,4 +406,9 @@ int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const 
     MX_GUARD(forward_mx(h, X, Wrouter, Wup, Wdown, Y, beta, tokens))
 }
 
+int tmt_moe_mxfp4_recorded(const tmt_moe* h) {
+    if (!h) { set_error("null handle"); return -1; }
+    return h->mx.recorded ? 1 : 0;
+}
+
 }  // extern "C"

@@ -37,7 +37,7 @@ EXPORTS = (
     "tmt_sampler_stream", "tmt_sampler_step", "tmt_sampler_upload", "tmt_sampler_download", "tmt_sampler_sync",
     "tmt_sampler_sample", "tmt_sampler_steps", "tmt_sampler_graphs", "tmt_sampler_set_layernorm",
     "tmt_moe_mxfp4_scale_bytes", "tmt_moe_quantize_mxfp4", "tmt_moe_dequantize_mxfp4", "tmt_moe_matmul_mxfp4",
-    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_act8_save", "tmt_moe_act8_restore",
+    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_mxfp4_recorded", "tmt_moe_act8_save", "tmt_moe_act8_restore",
     "tmt_ln_forward_act8", "tmt_ln_backward_act8", "tmt_ln_backward_act8_scratch_bytes",
 )
 
@@ -125,11 +125,13 @@ class MoE:
         self.tokens, self.dim, self.hidden, self.experts, self.topk = tokens, dim, hidden, experts, topk
         self.pad = 256 if gemm_impl in (GEMM_AUTO, GEMM_TCGEN05_2CTA) else 128      # rows every expert group is padded to
         self._keep = None
+        self._mx_keep, self._mx_recorded = None, {}
 
     def close(self):
         if getattr(self, "h", None) is not None and self.h.value:
             self.lib.tmt_moe_destroy(self.h)
             self.h = ctypes.c_void_p()
+            self._mx_keep, self._mx_recorded = None, {}
 
     def __del__(self):
         try:
@@ -251,7 +253,8 @@ class MoE:
 
     def forward_mxfp4(self, X, Wrouter, Wup, Wdown, Y, beta=0.0, tokens=None):
         """forward with both expert products on 4-bit blocks (include/tmt_mx.h). Wup / Wdown: Mxfp4Weights, or lists of
-        (codes, scales, rows, cols), one entry per expert (a Mxfp4Weights kept by the caller saves building it at every call)."""
+        (codes, scales, rows, cols), one entry per expert (a Mxfp4Weights kept by the caller saves building it at every call). The
+        handle keeps the weights of the last call alive, and those of calls that were recorded into a graph until it is closed."""
         t = self.tokens if tokens is None else tokens
         up = Wup if isinstance(Wup, Mxfp4Weights) else Mxfp4Weights(Wup)
         down = Wdown if isinstance(Wdown, Mxfp4Weights) else Mxfp4Weights(Wdown)
@@ -261,9 +264,19 @@ class MoE:
         if X.shape[-1] != self.dim or Y.shape[-1] != self.dim:
             raise MoeError("X and Y must have the handle's width, %d" % self.dim)
         _dense(Wrouter, "Wrouter", _FP if self.desc.router_dtype == F32 else _BF, self.experts * self.dim)
-        self._mx_keep = (up, down)          # the handle keeps a table of their device addresses
+        if self._mx_keep is None or self._mx_keep[0] is not up or self._mx_keep[1] is not down:
+            self._mx_change(up, down)
         if self.lib.tmt_moe_forward_mxfp4(self.h, X.data_ptr(), Wrouter.data_ptr(), up.arr, down.arr, Y.data_ptr(), beta, t):
             _check(-1, self.lib)
+
+    def _mx_change(self, up, down):
+        """The handle keeps a table of its weights' device addresses, and a graph the one it was recorded with."""
+        last = self._mx_keep
+        if last is not None:
+            key = bytes(last[0].arr), bytes(last[1].arr)
+            if key != (bytes(up.arr), bytes(down.arr)) and self.lib.tmt_moe_mxfp4_recorded(self.h):
+                self._mx_recorded[key] = last
+        self._mx_keep = (up, down)
 
     def nvfp4_weights_changed(self):
         """Call after re-quantising into the same buffers: derived copies are rebuilt at the next forward_nvfp4."""
@@ -520,7 +533,7 @@ def _declare_mx(lib):
             ("tmt_moe_mxfp4_scale_bytes", sz, [ll, i]), ("tmt_moe_linear_mxfp4_work_bytes", sz, [ll, i]),
             ("tmt_moe_quantize_mxfp4", i, [vp, i, ll, i, vp, vp, vp]), ("tmt_moe_dequantize_mxfp4", i, [vp, vp, ll, i, vp, i, vp]),
             ("tmt_moe_matmul_mxfp4", i, [vp, vp, i, wp, vp, i, vp, vp]), ("tmt_moe_linear_mxfp4", i, [vp, i, i, wp, vp, i, vp, sz, vp, vp]),
-            ("tmt_moe_forward_mxfp4", i, [vp, vp, vp, wp, wp, vp, f, i]),
+            ("tmt_moe_forward_mxfp4", i, [vp, vp, vp, wp, wp, vp, f, i]), ("tmt_moe_mxfp4_recorded", i, [vp]),
             ("tmt_moe_act8_save", i, [vp, i, ll, i, i, vp, vp, vp]), ("tmt_moe_act8_restore", i, [vp, vp, ll, i, i, vp, i, vp]),
             ("tmt_ln_forward_act8", i, [vp] * 8 + [i, i, i, vp]), ("tmt_ln_backward_act8_scratch_bytes", sz, [i, i]),
             ("tmt_ln_backward_act8", i, [vp, vp, i] + [vp] * 7 + [i, i, vp, vp])):

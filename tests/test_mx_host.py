@@ -65,3 +65,49 @@ def test_tables_of_weights_when_memory_runs_out(M, tmp_path):
     cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
     subprocess.run(["g++", "-std=c++17", "-I", csrc, "-I", cuda, str(src), "-o", str(tmp_path / "check")], check=True)
     subprocess.run([str(tmp_path / "check")], check=True)
+
+
+def test_the_front_end_keeps_recorded_weights_alive(M, monkeypatch):
+    """A graph goes on reading the weights it was recorded with, whatever later calls are given and the caller drops."""
+    import gc
+    import weakref
+    from test_front_end_dry_run import FakeLib
+
+    class Lib(FakeLib):
+        recorded = 0
+
+        def __getattr__(self, name):
+            if name == "tmt_moe_mxfp4_recorded":
+                return lambda h: self.recorded
+            return FakeLib.__getattr__(self, name)
+    lib = Lib()
+    monkeypatch.setattr(M, "_lib", lib)
+    E, D, H = 2, 64, 128
+    moe = M.MoE(8, D, E, 1, hidden=H, training=False)
+    X, Y, Wr = torch.zeros(8, D, dtype=torch.bfloat16), torch.zeros(8, D, dtype=torch.bfloat16), torch.zeros(E, D, dtype=torch.bfloat16)
+
+    def weights():
+        return [[(torch.zeros(n * k // 2, dtype=torch.uint8), torch.zeros(1024, dtype=torch.uint8), n, k) for _ in range(E)] for n, k in ((H, D), (D, H))]
+
+    def call(w):
+        moe.forward_mxfp4(X, Wr, w[0], w[1], Y)
+        return weakref.ref(w[0][0][0]), weakref.ref(w[1][E - 1][1])
+
+    def alive(refs):
+        gc.collect()
+        return [r() is not None for r in refs]
+    a = call(weights())
+    assert alive(a) == [True, True]                      # the handle's table points at them
+    lib.recorded = 1
+    b = call(weights())                                  # a was recorded, b is not
+    lib.recorded = 0
+    assert alive(a) == [True, True]
+    c = call(weights())
+    assert alive(a) == [True, True] and alive(b) == [False, False] and alive(c) == [True, True]
+    kept = M.Mxfp4Weights(weights()[0]), M.Mxfp4Weights(weights()[1])
+    lib.recorded = 1
+    for _ in range(3):
+        moe.forward_mxfp4(X, Wr, *kept, Y)               # c counts as recorded once, kept needs no entry while it is the last
+    assert len(moe._mx_recorded) == 2 and alive(c) == [True, True]
+    moe.close()
+    assert alive(a) + alive(c) == [False] * 4
