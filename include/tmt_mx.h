@@ -40,6 +40,9 @@ extern "C" {
 /* Formats of the 8-bit checkpoints. */
 enum { TMT_ACT8_E4M3 = 1, TMT_ACT8_E5M2 = 2 };
 
+/* Kernels of a 4-bit product: few rows per weight matrix, 128 x 128 tiles, CTA pairs on 256 x 256 tiles. */
+enum { TMT_MXFP4_FEW_ROWS = 0, TMT_MXFP4_TILES = 1, TMT_MXFP4_PAIRS = 2 };
+
 /* A 4-bit weight matrix W (rows = outputs, cols = inputs), [out,in] as everywhere in tmt_moe.h. */
 typedef struct tmt_mxfp4_weight {
     const void* codes;
@@ -68,6 +71,8 @@ int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, co
 size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols);
 int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
                          size_t work_bytes, int* status, void* stream);
+/* Which kernel the layer's product takes on the current device (for profiles and tests); -1 for a shape that is not supported. */
+int tmt_moe_linear_mxfp4_form(int rows, int n, int k);
 
 /* tmt_moe_forward with both expert products on 4-bit blocks (hidden > 0, training = 0, a single rank). The router, the gate
  * weights, the statistics and the residual (beta) are those of tmt_moe_forward, bit for bit; a token's row is quantised on its
@@ -81,6 +86,8 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
  * recorded with, whatever later calls are given. */
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
                           const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
+/* Which kernel the up (product 0) and the down product (1) of a call with `tokens` tokens take; -1 for arguments out of range. */
+int tmt_moe_forward_mxfp4_form(const tmt_moe* h, int tokens, int product);
 /* 1 when the weights last handed to tmt_moe_forward_mxfp4 were recorded into a graph (which goes on reading them), else 0; -1 for a
  * null handle. */
 int tmt_moe_mxfp4_recorded(const tmt_moe* h);

@@ -235,6 +235,13 @@ void refresh_tables(tmt_moe* h, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_wei
     m.key = key;
 }
 
+// The kernel of an expert product with n outputs and k inputs. With few rows per expert both products take the few-row kernel.
+int experts_form(const tmt_moe* h, int tokens, int n, int k) {
+    const long rows = (long)tokens * h->d.topk;
+    if (mx_decode_grouped(rows, h->d.experts, std::max(h->d.dim, h->d.hidden))) return TMT_MXFP4_FEW_ROWS;
+    return mx_form(rows, h->d.experts, n, k, h->num_sms, h->pad) == kMxPair ? TMT_MXFP4_PAIRS : TMT_MXFP4_TILES;
+}
+
 void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown, void* Y,
                 float beta, int tokens) {
     const int D = h->d.dim, H = h->d.hidden, E = h->d.experts, K = h->d.topk;
@@ -251,7 +258,7 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     h->dims.T = tokens;
     h->last_tokens = tokens;
     route_only(h, static_cast<const uint16_t*>(X), Wr);
-    if (mx_decode_grouped((long)tokens * K, E, std::max(D, H))) {
+    if (experts_form(h, tokens, H, D) == TMT_MXFP4_FEW_ROWS) {
         // Few rows per expert: no dispatch; up finds and quantises its rows itself and writes one row per assignment, down reads those.
         MxDecode q;
         memset(&q, 0, sizeof q);
@@ -289,13 +296,13 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
         p.w_scales_tab = m.scale_tab + (size_t)product * E;
     };
     p.n = H; p.k = D; p.epi = kMxUp; p.out = m.h_codes; p.out_scales = m.h_scales;
-    p.form = mx_form((long)tokens * K, E, p.n, p.k, h->num_sms, h->pad);
+    p.form = experts_form(h, tokens, p.n, p.k) == TMT_MXFP4_PAIRS ? kMxPair : kMxMany;
     p.act = m.x_map; p.act_scales = m.x_scales; p.act_sf = m.x_sf;
     weights(0);
     prof_mark(h, kPhGemmUp);
     cuda_ok(launch_mx_gemm(p, h->num_sms, h->stream), "mx up launch");
     p.n = D; p.k = H; p.epi = kMxDown; p.out = m.y_rows; p.out_scales = nullptr; p.out_map = m.y_out; p.row_scale = h->rb.slotw;
-    p.form = mx_form((long)tokens * K, E, p.n, p.k, h->num_sms, h->pad);
+    p.form = experts_form(h, tokens, p.n, p.k) == TMT_MXFP4_PAIRS ? kMxPair : kMxMany;
     p.act = m.h_map; p.act_scales = m.h_scales; p.act_sf = m.h_sf;
     weights(1);
     prof_mark(h, kPhGemmDown);
@@ -307,10 +314,19 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     h->have_forward = true;
 }
 
+void check_weight(int rows, int cols) {
+    if (rows < 8 || rows % 8 || cols < 64 || cols % 64) throw std::runtime_error("MXFP4 weight: rows must be a positive multiple of 8, cols of 64");
+}
 void check_weight(const tmt_mxfp4_weight* W) {
     if (!W) throw std::runtime_error("null argument");
-    if (W->rows < 8 || W->rows % 8 || W->cols < 64 || W->cols % 64)
-        throw std::runtime_error("MXFP4 weight: rows must be a positive multiple of 8, cols of 64");
+    check_weight(W->rows, W->cols);
+}
+
+// The kernel of a dense product; codes: the rows come as codes.
+int dense_form(int rows, int n, int k, bool codes) {
+    const int sms = sm_count();
+    if (mx_decode_dense(rows, k, mx_decode_split(n, k, sms), codes)) return TMT_MXFP4_FEW_ROWS;
+    return mx_form(rows, 1, n, k, sms, 256) == kMxPair ? TMT_MXFP4_PAIRS : TMT_MXFP4_TILES;
 }
 
 // Up to 32 rows, from values or from codes.
@@ -328,13 +344,14 @@ void few_rows(const void* src, const void* scales, int kind, int rows, const tmt
 }
 
 void matmul(const void* codes, const void* scales, int rows, const tmt_mxfp4_weight& W, void* Y, int dtype, int* status, cudaStream_t s) {
-    if (mx_decode_dense(rows, W.cols, mx_decode_split(W.rows, W.cols, sm_count()), true)) return few_rows(codes, scales, kMxSrcTiles, rows, W, Y, dtype, status, s);
+    const int form = dense_form(rows, W.rows, W.cols, true);
+    if (form == TMT_MXFP4_FEW_ROWS) return few_rows(codes, scales, kMxSrcTiles, rows, W, Y, dtype, status, s);
     MxGemm p;
     memset(&p, 0, sizeof p);
     const int sms = sm_count();
     p.rows = rows; p.n = W.rows; p.k = W.cols;
     p.epi = dtype == TMT_MOE_F32 ? kMxF32 : kMxBf16; p.out = Y; p.status = status;
-    p.form = mx_form(rows, 1, p.n, p.k, sms, 256);
+    p.form = form == TMT_MXFP4_PAIRS ? kMxPair : kMxMany;
     p.act_scales = static_cast<const uint8_t*>(scales); p.w_scales = static_cast<const uint8_t*>(W.scales);
     mx_make_map(&p.act, codes, rows, p.k, kMxBoxRows);
     mx_make_map(&p.w, W.codes, p.n, p.k, kMxBoxRows);
@@ -389,7 +406,7 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         check_tensors({X, W->codes, W->scales, Y, work});
         if (status) check_tensors({status}, 4);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (mx_decode_dense(rows, W->cols, mx_decode_split(W->rows, W->cols, sm_count()), false)) {
+        if (dense_form(rows, W->rows, W->cols, false) == TMT_MXFP4_FEW_ROWS) {
             few_rows(X, nullptr, x_dtype == TMT_MOE_F32 ? kMxSrcF32 : kMxSrcBf16, rows, *W, Y, y_dtype, status, s);
             return 0;
         }
@@ -398,6 +415,21 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         cuda_ok(launch_mx4_quantize(X, x_dtype == TMT_MOE_F32, rows, W->cols, codes, scales, s, true), "quantize_mxfp4 launch");
         matmul(codes, scales, rows, *W, Y, y_dtype, status, s);
     })
+}
+
+int tmt_moe_linear_mxfp4_form(int rows, int n, int k) {
+    try {
+        check_weight(n, k);
+        if (rows < 1) throw std::runtime_error("rows must be positive");
+        const int form = dense_form(rows, n, k, false);
+        return form == TMT_MXFP4_FEW_ROWS ? form : dense_form(rows, n, k, true);        // quantised first, then a product of codes
+    } catch (const std::exception& e) { set_error("%s", e.what()); return -1; }
+}
+
+int tmt_moe_forward_mxfp4_form(const tmt_moe* h, int tokens, int product) {
+    if (!h) { set_error("null handle"); return -1; }
+    if (tokens < 1 || tokens > h->d.tokens || product < 0 || product > 1) { set_error("tokens outside [1, desc.tokens], or product not 0 or 1"); return -1; }
+    return product == 0 ? experts_form(h, tokens, h->d.hidden, h->d.dim) : experts_form(h, tokens, h->d.dim, h->d.hidden);
 }
 
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup, const tmt_mxfp4_weight* Wdown,

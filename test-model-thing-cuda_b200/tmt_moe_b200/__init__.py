@@ -19,6 +19,7 @@ BF16, F32 = 0, 1
 GEMM_AUTO, GEMM_SIMT, GEMM_TCGEN05_2CTA, GEMM_TCGEN05 = 0, 1, 2, 3
 EP_PEER, EP_NCCL, EP_DMA = 0, 1, 2
 ACT8_E4M3, ACT8_E5M2 = 1, 2
+MXFP4_FEW_ROWS, MXFP4_TILES, MXFP4_PAIRS = 0, 1, 2
 
 EXPORTS = (
     "tmt_moe_create", "tmt_moe_destroy", "tmt_moe_last_error", "tmt_moe_set_router_bias",
@@ -37,7 +38,8 @@ EXPORTS = (
     "tmt_sampler_stream", "tmt_sampler_step", "tmt_sampler_upload", "tmt_sampler_download", "tmt_sampler_sync",
     "tmt_sampler_sample", "tmt_sampler_steps", "tmt_sampler_graphs", "tmt_sampler_set_layernorm",
     "tmt_moe_mxfp4_scale_bytes", "tmt_moe_quantize_mxfp4", "tmt_moe_dequantize_mxfp4", "tmt_moe_matmul_mxfp4",
-    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_mxfp4_recorded", "tmt_moe_act8_save", "tmt_moe_act8_restore",
+    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_mxfp4_recorded", "tmt_moe_linear_mxfp4_form",
+    "tmt_moe_forward_mxfp4_form", "tmt_moe_act8_save", "tmt_moe_act8_restore",
     "tmt_ln_forward_act8", "tmt_ln_backward_act8", "tmt_ln_backward_act8_scratch_bytes",
 )
 
@@ -268,6 +270,10 @@ class MoE:
             self._mx_change(up, down)
         if self.lib.tmt_moe_forward_mxfp4(self.h, X.data_ptr(), Wrouter.data_ptr(), up.arr, down.arr, Y.data_ptr(), beta, t):
             _check(-1, self.lib)
+
+    def forward_mxfp4_form(self, product, tokens=None):
+        """Which kernel the up (0) or down product (1) of forward_mxfp4 takes: MXFP4_FEW_ROWS, MXFP4_TILES or MXFP4_PAIRS."""
+        return _form(self.lib, self.lib.tmt_moe_forward_mxfp4_form(self.h, self.tokens if tokens is None else tokens, product))
 
     def _mx_change(self, up, down):
         """The handle keeps a table of its weights' device addresses, and a graph the one it was recorded with."""
@@ -534,6 +540,7 @@ def _declare_mx(lib):
             ("tmt_moe_quantize_mxfp4", i, [vp, i, ll, i, vp, vp, vp]), ("tmt_moe_dequantize_mxfp4", i, [vp, vp, ll, i, vp, i, vp]),
             ("tmt_moe_matmul_mxfp4", i, [vp, vp, i, wp, vp, i, vp, vp]), ("tmt_moe_linear_mxfp4", i, [vp, i, i, wp, vp, i, vp, sz, vp, vp]),
             ("tmt_moe_forward_mxfp4", i, [vp, vp, vp, wp, wp, vp, f, i]), ("tmt_moe_mxfp4_recorded", i, [vp]),
+            ("tmt_moe_linear_mxfp4_form", i, [i, i, i]), ("tmt_moe_forward_mxfp4_form", i, [vp, i, i]),
             ("tmt_moe_act8_save", i, [vp, i, ll, i, i, vp, vp, vp]), ("tmt_moe_act8_restore", i, [vp, vp, ll, i, i, vp, i, vp]),
             ("tmt_ln_forward_act8", i, [vp] * 8 + [i, i, i, vp]), ("tmt_ln_backward_act8_scratch_bytes", sz, [i, i]),
             ("tmt_ln_backward_act8", i, [vp, vp, i] + [vp] * 7 + [i, i, vp, vp])):
@@ -657,6 +664,18 @@ def matmul_mxfp4(codes, scales, W, Y, status=None, stream=None):
 
 def linear_mxfp4_work_bytes(rows, cols):
     return int(load().tmt_moe_linear_mxfp4_work_bytes(rows, cols))
+
+
+def _form(lib, form):
+    if form < 0:
+        _check(-1, lib)
+    return form
+
+
+def linear_mxfp4_form(rows, n, k):
+    """Which kernel linear_mxfp4 takes for X (rows, k) and a weight (n, k): MXFP4_FEW_ROWS, MXFP4_TILES or MXFP4_PAIRS."""
+    lib = _lib or load()
+    return _form(lib, lib.tmt_moe_linear_mxfp4_form(rows, n, k))
 
 
 def linear_mxfp4(X, W, Y, work, status=None, stream=None):

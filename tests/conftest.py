@@ -13,6 +13,16 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on the B200 box)")
 
 
+@pytest.fixture(autouse=True)
+def _gpu_idle_after(request):
+    """A GPU test's work is done before the next test takes its memory, and a fault names the test it belongs to."""
+    yield
+    if request.node.get_closest_marker("gpu"):
+        import torch
+        if torch.cuda.is_available():
+            torch.cuda.synchronize()
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle import oracle as o
