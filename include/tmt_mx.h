@@ -61,8 +61,9 @@ int tmt_moe_dequantize_mxfp4(const void* codes, const void* scales, long long ro
 
 /* Y = A W^T with both operands in 4-bit blocks, on the block-scaled tensor-core instruction: products exact, sums in fp32,
  * rounded once to `dtype`. A (rows, W->cols), Y (rows, W->rows) row-major and dense; W->rows: a multiple of 8, W->cols: a
- * multiple of 64. How k is shared among blocks depends on `rows`, and with it the last bits of a sum. status (device int, may
- * be NULL): receives a code of tmt_moe_device_status when a bounded wait ran out; never cleared here. */
+ * multiple of 64. How k is shared among blocks depends on `rows`, and with it the last bits of a sum. status (device int):
+ * receives a code of tmt_moe_device_status when a bounded wait ran out (Y is then not complete); never cleared here. NULL: the
+ * library's own word of the device receives it, see tmt_moe_mxfp4_status. */
 int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, const tmt_mxfp4_weight* W, void* Y, int dtype,
                          int* status, void* stream);
 
@@ -71,6 +72,12 @@ int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, co
 size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols);
 int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
                          size_t work_bytes, int* status, void* stream);
+/* The first code that a product without a status word of its own has recorded on the current device since the last call of this
+ * function, 0 when there is none; -1 on an error. Waits for the device, and clears the word. */
+int tmt_moe_mxfp4_status(void);
+/* Failure-detection self-test of that word: queues one block that waits on a barrier nothing arrives on, limit_cycles clock cycles
+ * long, through the same bounded wait as the products. tmt_moe_mxfp4_status then gives 2. */
+int tmt_moe_mxfp4_selftest_bounded_wait(long long limit_cycles, void* stream);
 /* Which kernel the layer's product takes on the current device (for profiles and tests); -1 for a shape that is not supported. */
 int tmt_moe_linear_mxfp4_form(int rows, int n, int k);
 

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <initializer_list>
 #include <stdexcept>
@@ -30,11 +31,27 @@ inline void check_tensors(std::initializer_list<const void*> ptrs, uintptr_t ali
     }
 }
 
-inline int sm_count() {
-    int dev = 0, sms = 0;
+// What the calls ask of the current device again and again, asked for once per device: `ask` fills in a value, which is not 0.
+template <class T, class Ask>
+T per_device(std::atomic<T> (&known)[64], Ask ask) {
+    int dev = 0;
     cuda_ok(cudaGetDevice(&dev), "cudaGetDevice");
-    cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
-    return sms;
+    if (dev < 64) {
+        const T v = known[dev].load(std::memory_order_acquire);
+        if (v) return v;
+    }
+    const T v = ask(dev);
+    if (dev < 64) known[dev].store(v, std::memory_order_release);
+    return v;
+}
+
+inline int sm_count() {
+    static std::atomic<int> known[64];
+    return per_device(known, [](int dev) {
+        int sms = 0;
+        cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+        return sms;
+    });
 }
 
 }  // namespace tmt

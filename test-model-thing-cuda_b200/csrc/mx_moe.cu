@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "../../include/tmt_mx.h"
+#include "gemm.cuh"
 #include "launch_pdl.cuh"
 #include "moe_internal.h"
 #include "mx.cuh"
@@ -19,6 +20,19 @@ namespace tmt {
 namespace {
 
 using namespace mx;
+
+// The status of products that are given no word of their own; the second word is where the self-test's kernel says it ended.
+__device__ int g_status[2];
+
+// Their address on the current device.
+int* shared_status() {
+    static std::atomic<int*> known[64];
+    return per_device(known, [](int) {
+        void* p = nullptr;
+        cuda_ok(cudaGetSymbolAddress(&p, g_status), "cudaGetSymbolAddress");
+        return static_cast<int*>(p);
+    });
+}
 
 constexpr int kDispatchWarps = 8;
 constexpr int kMaxTopk = 8;
@@ -386,6 +400,7 @@ int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, co
         if (rows == 0) return 0;
         check_tensors({A_codes, A_scales, W->codes, W->scales, Y});
         if (status) check_tensors({status}, 4);
+        else status = shared_status();
         matmul(A_codes, A_scales, rows, *W, Y, dtype, status, static_cast<cudaStream_t>(stream));
     })
 }
@@ -405,6 +420,7 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         if (work_bytes < tmt_moe_linear_mxfp4_work_bytes(rows, W->cols)) throw std::runtime_error("work buffer too small (tmt_moe_linear_mxfp4_work_bytes)");
         check_tensors({X, W->codes, W->scales, Y, work});
         if (status) check_tensors({status}, 4);
+        else status = shared_status();
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (dense_form(rows, W->rows, W->cols, false) == TMT_MXFP4_FEW_ROWS) {
             few_rows(X, nullptr, x_dtype == TMT_MOE_F32 ? kMxSrcF32 : kMxSrcBf16, rows, *W, Y, y_dtype, status, s);
@@ -414,6 +430,25 @@ int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_w
         uint8_t* scales = codes + codes_bytes(rows, W->cols);
         cuda_ok(launch_mx4_quantize(X, x_dtype == TMT_MOE_F32, rows, W->cols, codes, scales, s, true), "quantize_mxfp4 launch");
         matmul(codes, scales, rows, *W, Y, y_dtype, status, s);
+    })
+}
+
+int tmt_moe_mxfp4_status(void) {
+    try {
+        int* word = shared_status();
+        int v = 0;
+        cuda_ok(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+        cuda_ok(cudaMemcpy(&v, word, sizeof v, cudaMemcpyDeviceToHost), "cudaMemcpy");
+        if (v) cuda_ok(cudaMemset(word, 0, sizeof v), "cudaMemset");
+        return v;
+    } catch (const std::exception& e) { set_error("%s", e.what()); return -1; }
+}
+
+int tmt_moe_mxfp4_selftest_bounded_wait(long long limit_cycles, void* stream) {
+    MX_GUARD({
+        if (limit_cycles < 1 || limit_cycles > 2000000000LL) throw std::runtime_error("limit_cycles outside [1, 2e9]");
+        int* words = shared_status();
+        cuda_ok(launch_bounded_wait_selftest(words, limit_cycles, words + 1, static_cast<cudaStream_t>(stream)), "self-test launch");
     })
 }
 

@@ -38,7 +38,8 @@ EXPORTS = (
     "tmt_sampler_stream", "tmt_sampler_step", "tmt_sampler_upload", "tmt_sampler_download", "tmt_sampler_sync",
     "tmt_sampler_sample", "tmt_sampler_steps", "tmt_sampler_graphs", "tmt_sampler_set_layernorm",
     "tmt_moe_mxfp4_scale_bytes", "tmt_moe_quantize_mxfp4", "tmt_moe_dequantize_mxfp4", "tmt_moe_matmul_mxfp4",
-    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_mxfp4_recorded", "tmt_moe_linear_mxfp4_form",
+    "tmt_moe_linear_mxfp4_work_bytes", "tmt_moe_linear_mxfp4", "tmt_moe_forward_mxfp4", "tmt_moe_mxfp4_recorded", "tmt_moe_mxfp4_status",
+    "tmt_moe_mxfp4_selftest_bounded_wait", "tmt_moe_linear_mxfp4_form",
     "tmt_moe_forward_mxfp4_form", "tmt_moe_act8_save", "tmt_moe_act8_restore",
     "tmt_ln_forward_act8", "tmt_ln_backward_act8", "tmt_ln_backward_act8_scratch_bytes",
 )
@@ -540,6 +541,7 @@ def _declare_mx(lib):
             ("tmt_moe_quantize_mxfp4", i, [vp, i, ll, i, vp, vp, vp]), ("tmt_moe_dequantize_mxfp4", i, [vp, vp, ll, i, vp, i, vp]),
             ("tmt_moe_matmul_mxfp4", i, [vp, vp, i, wp, vp, i, vp, vp]), ("tmt_moe_linear_mxfp4", i, [vp, i, i, wp, vp, i, vp, sz, vp, vp]),
             ("tmt_moe_forward_mxfp4", i, [vp, vp, vp, wp, wp, vp, f, i]), ("tmt_moe_mxfp4_recorded", i, [vp]),
+            ("tmt_moe_mxfp4_status", i, []), ("tmt_moe_mxfp4_selftest_bounded_wait", i, [ll, vp]),
             ("tmt_moe_linear_mxfp4_form", i, [i, i, i]), ("tmt_moe_forward_mxfp4_form", i, [vp, i, i]),
             ("tmt_moe_act8_save", i, [vp, i, ll, i, i, vp, vp, vp]), ("tmt_moe_act8_restore", i, [vp, vp, ll, i, i, vp, i, vp]),
             ("tmt_ln_forward_act8", i, [vp] * 8 + [i, i, i, vp]), ("tmt_ln_backward_act8_scratch_bytes", sz, [i, i]),
@@ -635,6 +637,16 @@ def _status(t):
     return t.data_ptr()
 
 
+def mxfp4_status():
+    """First code that a linear_mxfp4 or matmul_mxfp4 without a status tensor has recorded on the current device since the last call
+    (2: a bounded wait ran out, its output is not complete), 0 when there is none. Waits for the device."""
+    lib = _lib or load()
+    code = lib.tmt_moe_mxfp4_status()
+    if code < 0:
+        _check(-1, lib)
+    return code
+
+
 def _one_weight(W):
     W = W if isinstance(W, Mxfp4Weights) else Mxfp4Weights([W])
     if W.n != 1:
@@ -650,7 +662,8 @@ def _out(Y, rows, W):
 
 
 def matmul_mxfp4(codes, scales, W, Y, status=None, stream=None):
-    """Y (rows, W rows) = A W^T, both in 4-bit blocks; W: Mxfp4Weights with one entry, or (codes, scales, rows, cols)."""
+    """Y (rows, W rows) = A W^T, both in 4-bit blocks; W: Mxfp4Weights with one entry, or (codes, scales, rows, cols). status: an int32
+    tensor that receives the code of a wait that ran out; without one mxfp4_status() tells."""
     lib = _lib or load()
     W = _one_weight(W)
     rows, k = Y.shape[0], W.cols
@@ -679,7 +692,8 @@ def linear_mxfp4_form(rows, n, k):
 
 
 def linear_mxfp4(X, W, Y, work, status=None, stream=None):
-    """Y = q4(X) W^T: X (rows, cols) bf16 or fp32 is quantised into work (linear_mxfp4_work_bytes(rows, cols) bytes) and multiplied."""
+    """Y = q4(X) W^T: X (rows, cols) bf16 or fp32 is quantised into work (linear_mxfp4_work_bytes(rows, cols) bytes) and multiplied.
+    status as in matmul_mxfp4."""
     lib = _lib or load()
     W = _one_weight(W)
     rows, k = _matrix(X, "X")

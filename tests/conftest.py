@@ -15,12 +15,15 @@ def pytest_configure(config):
 
 @pytest.fixture(autouse=True)
 def _gpu_idle_after(request):
-    """A GPU test's work is done before the next test takes its memory, and a fault names the test it belongs to."""
+    """A GPU test's work is done before the next test takes its memory, and a fault or a wait that ran out names the test it belongs to."""
     yield
     if request.node.get_closest_marker("gpu"):
         import torch
         if torch.cuda.is_available():
             torch.cuda.synchronize()
+            import tmt_moe_b200 as M
+            if M._lib is not None:
+                assert M.mxfp4_status() == 0           # no product gave up waiting
 
 
 @pytest.fixture(scope="session")
