@@ -581,10 +581,20 @@ def _dense(t, name, kinds, need):
 _VALUES, _BF, _FP, _BY = (BF16, F32), (BF16,), (F32,), (_BYTE,)
 
 
-def _matrix(t, name):
+_INT_MAX = 2 ** 31 - 1
+
+
+def _matrix(t, name, rows_max=_INT_MAX):
+    """(rows, cols) of a matrix, refused where the library's argument would wrap around."""
     if t.dim() != 2:
         raise MoeError("%s must have two dimensions" % name)
-    return t.shape
+    rows, cols = t.shape
+    if rows > rows_max or cols > _INT_MAX:
+        raise MoeError("%s has shape %s: more rows or columns than are supported" % (name, (rows, cols)))
+    return rows, cols
+
+
+_ANY_ROWS = 2 ** 63 - 1     # the casts count rows in 64 bits
 
 
 class Mxfp4Weights:
@@ -596,6 +606,8 @@ class Mxfp4Weights:
         self.n = len(entries)
         self.arr = (_Mxfp4WeightDesc * self.n)()
         for i, (c, s, r, k) in enumerate(entries):
+            if not (0 < r <= _INT_MAX and 0 < k <= _INT_MAX):
+                raise MoeError("a weight of shape %s is not supported" % ((r, k),))
             _dense(c, "codes", _BY, r * k // 2)
             _dense(s, "scales", _BY, mxfp4_scale_bytes(r, k))
             self.arr[i] = _Mxfp4WeightDesc(c.data_ptr(), s.data_ptr(), r, k)
@@ -610,7 +622,7 @@ def mxfp4_scale_bytes(rows, cols):
 def quantize_mxfp4(X, codes, scales, stream=None):
     """X (rows, cols) bf16 or fp32 -> 4-bit blocks; codes: rows * cols / 2 bytes, scales: mxfp4_scale_bytes(rows, cols) bytes."""
     lib = _lib or load()
-    rows, cols = _matrix(X, "X")
+    rows, cols = _matrix(X, "X", _ANY_ROWS)
     dt = _dense(X, "X", _VALUES, 0)
     _dense(codes, "codes", _BY, rows * cols // 2)
     _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
@@ -621,7 +633,7 @@ def quantize_mxfp4(X, codes, scales, stream=None):
 def dequantize_mxfp4(codes, scales, Y, stream=None):
     """4-bit blocks -> Y (rows, cols) bf16 or fp32."""
     lib = _lib or load()
-    rows, cols = _matrix(Y, "Y")
+    rows, cols = _matrix(Y, "Y", _ANY_ROWS)
     dt = _dense(Y, "Y", _VALUES, 0)
     _dense(codes, "codes", _BY, rows * cols // 2)
     _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, cols))
@@ -666,7 +678,7 @@ def matmul_mxfp4(codes, scales, W, Y, status=None, stream=None):
     tensor that receives the code of a wait that ran out; without one mxfp4_status() tells."""
     lib = _lib or load()
     W = _one_weight(W)
-    rows, k = Y.shape[0], W.cols
+    rows, k = _matrix(Y, "Y")[0], W.cols
     dt = _out(Y, rows, W)
     _dense(codes, "codes", _BY, rows * k // 2)
     _dense(scales, "scales", _BY, lib.tmt_moe_mxfp4_scale_bytes(rows, k))
@@ -709,7 +721,7 @@ def linear_mxfp4(X, W, Y, work, status=None, stream=None):
 def act8_save(X, codes, scales, fmt=ACT8_E4M3, stream=None):
     """8-bit checkpoint of X (rows, cols) bf16 or fp32; codes: rows * cols bytes, scales: rows * cols / 32 bytes."""
     lib = _lib or load()
-    rows, cols = _matrix(X, "X")
+    rows, cols = _matrix(X, "X", _ANY_ROWS)
     dt = _dense(X, "X", _VALUES, 0)
     _dense(codes, "codes", _BY, rows * cols)
     _dense(scales, "scales", _BY, rows * cols // 32)
@@ -720,7 +732,7 @@ def act8_save(X, codes, scales, fmt=ACT8_E4M3, stream=None):
 def act8_restore(codes, scales, Y, fmt=ACT8_E4M3, stream=None):
     """The values of an 8-bit checkpoint -> Y (rows, cols) bf16 or fp32."""
     lib = _lib or load()
-    rows, cols = _matrix(Y, "Y")
+    rows, cols = _matrix(Y, "Y", _ANY_ROWS)
     dt = _dense(Y, "Y", _VALUES, 0)
     _dense(codes, "codes", _BY, rows * cols)
     _dense(scales, "scales", _BY, rows * cols // 32)

@@ -111,3 +111,27 @@ def test_the_front_end_keeps_recorded_weights_alive(M, monkeypatch):
     assert len(moe._mx_recorded) == 2 and alive(c) == [True, True]
     moe.close()
     assert alive(a) + alive(c) == [False] * 4
+
+
+def test_the_front_end_refuses_sizes_that_would_wrap(M, monkeypatch):
+    """A size past 32 bits reaches a C int as its low half: a matrix of 2^32 + 64 columns would be taken for one of 64."""
+    from test_front_end_dry_run import FakeLib
+    monkeypatch.setattr(M, "_lib", FakeLib())            # accepts whatever it is given
+
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+    n = 2 ** 32 + 64
+    by = meta(2 ** 40, dtype=torch.uint8)
+    f = meta(2 ** 40, dtype=torch.float32)
+    W = (by, by, 8, 64)
+    wide, tall, y = meta(1, n), meta(n, 64), meta(n, 8)
+    calls = [lambda: M.quantize_mxfp4(wide, by, by), lambda: M.dequantize_mxfp4(by, by, wide), lambda: M.act8_save(wide, by, by),
+             lambda: M.act8_restore(by, by, wide), lambda: M.linear_mxfp4(tall, W, y, by), lambda: M.matmul_mxfp4(by, by, W, y),
+             lambda: M.ln_forward_act8(tall, f, f, tall, f, f, by, by), lambda: M.ln_forward_act8(wide, f, f, wide, f, f, by, by),
+             lambda: M.ln_backward_act8(by, by, tall, f, f, f, tall, f, f, by), lambda: M.linear_mxfp4(meta(4, 64), (by, by, n, 64), meta(4, n), by),
+             lambda: M.Mxfp4Weights([(by, by, 8, n)]), lambda: M.Mxfp4Weights([(by, by, -8, 64)]), lambda: M.matmul_mxfp4(by, by, W, meta())]
+    for call in calls:
+        with pytest.raises(M.MoeError):
+            call()
+    M.quantize_mxfp4(tall, by, by)                       # the casts count rows in 64 bits
+    M.act8_restore(by, by, tall)
