@@ -61,9 +61,9 @@ int tmt_moe_dequantize_mxfp4(const void* codes, const void* scales, long long ro
 
 /* Y = A W^T with both operands in 4-bit blocks, on the block-scaled tensor-core instruction: products exact, sums in fp32,
  * rounded once to `dtype`. A (rows, W->cols), Y (rows, W->rows) row-major and dense; W->rows: a multiple of 8, W->cols: a
- * multiple of 64. How k is shared among blocks depends on `rows`, and with it the last bits of a sum. status (device int):
- * receives a code of tmt_moe_device_status when a bounded wait ran out (Y is then not complete); never cleared here. NULL: the
- * library's own word of the device receives it, see tmt_moe_mxfp4_status. */
+ * multiple of 64, at most 2^28. How k is shared among blocks depends on `rows`, and with it the last bits of a sum. status
+ * (device int): receives a code of tmt_moe_device_status when a bounded wait ran out (Y is then not complete); never cleared
+ * here. NULL: the library's own word of the device receives it, see tmt_moe_mxfp4_status. */
 int tmt_moe_matmul_mxfp4(const void* A_codes, const void* A_scales, int rows, const tmt_mxfp4_weight* W, void* Y, int dtype,
                          int* status, void* stream);
 

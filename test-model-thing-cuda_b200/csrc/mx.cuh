@@ -90,7 +90,9 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t w, float (&f)[8]) {
 // (row % 32) * 16 + (row % 128 / 32) * 4 + block % 4, copied to tensor memory as it is. A matrix keeps them in that
 // order: tiles of a 128-row band one after the other, band after band; rows and blocks are padded to whole tiles.
 constexpr int kScaleTile = 512;
-__host__ __device__ __forceinline__ int scale_tiles_k(int cols) { return (cols + 127) / 128; }
+// Sizes go up to the end of the int range, so rounding up starts from one less. a >= 1.
+__host__ __device__ __forceinline__ constexpr int ceil_div(int a, int b) { return (a - 1) / b + 1; }
+__host__ __device__ __forceinline__ int scale_tiles_k(int cols) { return ceil_div(cols, 128); }
 __host__ __device__ __forceinline__ size_t scale_bytes(long rows, int cols) {
     return (size_t)((rows + 127) / 128) * scale_tiles_k(cols) * kScaleTile;
 }

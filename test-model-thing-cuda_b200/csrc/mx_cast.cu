@@ -168,7 +168,7 @@ struct Grid { unsigned chunks, per_row; int u; dim3 grid; };
 // bands: chunks are counted over 32 rows of every band of 128 (4-bit quantiser: a warp takes four rows of a band at once)
 Grid plan(long long rows, int cols, bool bands = false) {
     Grid g;
-    g.per_row = (unsigned)((cols + kChunk - 1) / kChunk);
+    g.per_row = (unsigned)ceil_div(cols, kChunk);
     if (rows > 0x7fffffffLL / g.per_row) throw std::runtime_error("rows * cols exceeds the supported range");
     if (bands) {
         const long long r = rows / 128 * 32 + (rows % 128 < 32 ? rows % 128 : 32);

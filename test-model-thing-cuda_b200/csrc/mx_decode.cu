@@ -220,10 +220,10 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
     __shared__ int abort_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int w_tiles = (p.n + 127) >> 7;
+    const int w_tiles = ceil_div(p.n, 128);
     const int split = SPLIT ? p.split : 1, part = SPLIT ? (int)blockIdx.x % split : 0, tile = SPLIT ? (int)blockIdx.x / split : (int)blockIdx.x;
     const int e = SPLIT ? 0 : tile / w_tiles, w0 = (SPLIT ? tile : tile % w_tiles) << 7;
-    const int nkb_all = (p.k + kKB - 1) / kKB;
+    const int nkb_all = ceil_div(p.k, kKB);
     const int kb0 = SPLIT ? nkb_all * part / split : 0, nkb = SPLIT ? nkb_all * (part + 1) / split - kb0 : nkb_all;      // this block's share of k
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t codes_w = base, act = codes_w + stages * kCodesW, sf_w = act + nkb * kStageA;      // 1024-byte multiples throughout
@@ -399,14 +399,14 @@ __global__ void __launch_bounds__(kThreads, 2) mx_decode_kernel(const __grid_con
 
 template <int SRC, int EPI, bool SPLIT>
 cudaError_t launch_t(const MxDecode& p, cudaStream_t stream) {
-    const int nkb = ((p.k + kKB - 1) / kKB + p.split - 1) / p.split;      // the largest share
+    const int nkb = ceil_div(ceil_div(p.k, kKB), p.split);      // the largest share
     const int room = (kSmemMax - 1024 - nkb * kStageA) / kStageW;
     const int stages = room < nkb ? (room < kMaxStages ? room : kMaxStages) : (nkb < kMaxStages ? nkb : kMaxStages);
     const size_t smem = 1024 + (size_t)nkb * kStageA + (size_t)stages * kStageW;
     const auto kernel = mx_decode_kernel<SRC, EPI, SPLIT>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return e;
-    const int blocks = ((p.n + 127) / 128) * (p.experts ? p.experts : p.split);
+    const int blocks = ceil_div(p.n, 128) * (p.experts ? p.experts : p.split);
     if constexpr (!SPLIT) return launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, stream, p, stages);
     // a cluster per tile
     cudaLaunchConfig_t cfg = {};
@@ -432,9 +432,9 @@ cudaError_t launch_dense(const MxDecode& p, cudaStream_t stream) {
 //     1024 x 4096    9.8     5.7               1024 x 8192   15.8     6.4
 // Below 2048 a block alone is done sooner than any cluster was (1024 x 1024: 4.2): it starts early, which clusters go without.
 int mx_decode_split(int n, int k, int num_sms) {
-    const int tiles = (n + 127) / 128, nkb = (k + kKB - 1) / kKB;
+    const int tiles = ceil_div(n, 128), nkb = ceil_div(k, kKB);
     int split = 1;
-    while (split < 8 && nkb >= 8 && 4 * split <= nkb && 2 * split * tiles <= num_sms) split *= 2;
+    while (split < 8 && nkb >= 8 && 4 * split <= nkb && tiles <= num_sms / (2 * split)) split *= 2;
     return split;
 }
 
@@ -448,7 +448,7 @@ int mx_decode_split(int n, int k, int num_sms) {
 //     2048 -> 2048   5.7   6.0   6.5   7.1   7.4 |  5.4         8192 -> 1024   6.4   6.8   7.6   8.3   9.0 | 13.2
 bool mx_decode_dense(long rows, int k, int split, bool codes) {
     if (k > kMxDecodeMaxK || rows > kMxDecodeRows) return false;
-    const long nkb = (k + kKB - 1) / kKB, work = rows * ((nkb + split - 1) / split);
+    const long nkb = ceil_div(k, kKB), work = rows * ((nkb + split - 1) / split);
     if (codes) return split > 1 && work <= 8 * nkb - 64;
     return work <= (split > 1 ? 8 * nkb - 24 : 40);
 }
@@ -457,7 +457,7 @@ bool mx_decode_dense(long rows, int k, int split, bool codes) {
 //     16 experts 1024 -> 2048:   2 rows 26.6 | 33.8     8 rows 29.8 | 34.2    16 rows 41.6 | 38.4
 //      4 experts  512 -> 1024:   2 rows 21.2 | 25.5     8 rows 22.1 | 26.4    32 rows 32.1 | 26.3
 bool mx_decode_grouped(long rows, int groups, int k) {
-    const long nkb = (k + kKB - 1) / kKB;
+    const long nkb = ceil_div(k, kKB);
     return rows <= kMxDecodeMaxAsg && k <= kMxDecodeMaxK && rows <= 20L * groups && rows * nkb <= 80L * groups;
 }
 

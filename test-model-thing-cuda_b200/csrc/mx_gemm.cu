@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-    const int w_tiles = (p.n + TW - 1) / TW;
-    const int nkb = (p.k + kKB - 1) / kKB;
+    const int w_tiles = ceil_div(p.n, TW);
+    const int nkb = ceil_div(p.k, kKB);
     const int tiles_k = scale_tiles_k(p.k);
 
     if (warp == 0 || warp == 10) {
@@ -324,7 +324,7 @@ EncodeTiledFn encode_fn() {
 //     4096 -> 4096    128: 11.3 / 13.1    256: 19.0 / 14.3    384: 25.1 / 20.6    1024: 53.7 / 37.2
 int mx_form(long rows, int groups, int n, int k, int num_sms, int pad) {
     const long each = (rows + groups - 1) / groups;
-    const long tiles = groups * ((each + 127) / 128) * ((n + 127) / 128);
+    const long tiles = groups * ((each + 127) / 128) * (long)ceil_div(n, 128);
     return pad % 256 == 0 && tiles > (k >= 2048 ? 1 : 3) * num_sms ? kMxPair : kMxMany;
 }
 

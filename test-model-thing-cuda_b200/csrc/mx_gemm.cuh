@@ -32,7 +32,7 @@ struct Tile {
 template <int TA>                        // activation rows of a tile
 __device__ __forceinline__ void load_groups(const MxGemm& p, Groups& g) {
     if (p.experts == 0) {
-        if (threadIdx.x == 0) { g.first[0] = 0; g.first[1] = (p.rows - 1) / TA + 1; g.poff[0] = 0; g.count[0] = p.rows; }
+        if (threadIdx.x == 0) { g.first[0] = 0; g.first[1] = ceil_div(p.rows, TA); g.poff[0] = 0; g.count[0] = p.rows; }
         return;
     }
     for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {

@@ -124,8 +124,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx_gemm
     cluster_sync();            // both hold their tensor memory
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-    const int w_tiles = (p.n + kCols - 1) / kCols;
-    const int nkb = (p.k + kKB - 1) / kKB;
+    const int w_tiles = ceil_div(p.n, kCols);
+    const int nkb = ceil_div(p.k, kKB);
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
     // Loop control of the producers and of the MMA warp goes through warp votes: the compiler then knows it to be uniform and

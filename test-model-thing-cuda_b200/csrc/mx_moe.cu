@@ -328,8 +328,11 @@ void forward_mx(tmt_moe* h, const void* X, const void* Wr, const tmt_mxfp4_weigh
     h->have_forward = true;
 }
 
+// A tile's sum over k is one chain of about 0.3 us per 256, and the epilogue's wait for it is bounded (two seconds): 2^28 take 0.3 s.
+constexpr int kMaxK = 1 << 28;
 void check_weight(int rows, int cols) {
     if (rows < 8 || rows % 8 || cols < 64 || cols % 64) throw std::runtime_error("MXFP4 weight: rows must be a positive multiple of 8, cols of 64");
+    if (cols > kMaxK) throw std::runtime_error("MXFP4 weight: cols must be at most " + std::to_string(kMaxK));
 }
 void check_weight(const tmt_mxfp4_weight* W) {
     if (!W) throw std::runtime_error("null argument");

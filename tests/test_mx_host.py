@@ -135,3 +135,19 @@ def test_the_front_end_refuses_sizes_that_would_wrap(M, monkeypatch):
             call()
     M.quantize_mxfp4(tall, by, by)                       # the casts count rows in 64 bits
     M.act8_restore(by, by, tall)
+
+
+def test_sizes_at_the_end_of_the_column_range(M):
+    k = 2 ** 31 - 64
+    assert M.mxfp4_scale_bytes(1, k) == M.mxfp4_scale_bytes(128, k) == 2 ** 24 * 512
+    assert M.linear_mxfp4_work_bytes(1, k) == k // 2 + 2 ** 24 * 512
+
+
+def test_products_refuse_a_k_whose_sum_outlasts_the_bounded_waits(M):
+    import ctypes
+    lib, p = M.load(), 1 << 20
+    for k in (2 ** 28 + 64, 2 ** 31 - 64):
+        W = M._Mxfp4WeightDesc(p, p, 8, k)
+        for rc in (lib.tmt_moe_matmul_mxfp4(p, p, 4, ctypes.byref(W), p, 0, None, None),
+                   lib.tmt_moe_linear_mxfp4(p, 0, 4, ctypes.byref(W), p, 0, p, 1 << 62, None, None), lib.tmt_moe_linear_mxfp4_form(4, 8, k)):
+            assert rc == -1 and b"at most" in lib.tmt_moe_last_error()
