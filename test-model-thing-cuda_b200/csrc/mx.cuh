@@ -85,6 +85,41 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t w, float (&f)[8]) {
         asm("{\n\t.reg .f16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, u;\n\t}" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(h[i]));
 }
 
+// 8 values of a row (16 bytes of bf16, 32 of fp32) as floats; returns the fp32 bits of the largest magnitude among them
+__device__ __forceinline__ uint32_t spread8(const uint4& a, float (&f)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    uint32_t m = 0;                                           // two 16-bit maxima: magnitudes of bf16 order like their bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); m = __vmaxu2(m, w[i] & 0x7fff7fffu); }
+    return max(m >> 16, m & 0xffffu) << 16;
+}
+__device__ __forceinline__ uint32_t spread8(const uint4& a, const uint4& b, float (&f)[8]) {
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { f[i] = __uint_as_float(w[i]); m = max(m, w[i] & 0x7fffffffu); }
+    return m;
+}
+// Scale byte of a block held by 4 neighbouring lanes, 8 elements each, which are brought to units of the scale; m: the lane's largest.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_block(float (&f)[8], uint32_t m) {
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t sb = scale_byte<FMT>(m);
+    const float inv = inv_scale(sb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= inv;
+    return sb;
+}
+// The lane's 8 codes, and the word of scale bytes of the 4 blocks its 16 lanes hold (blocks of lanes that are not ok: 0).
+__device__ __forceinline__ uint32_t quantize8_e2m1(float (&f)[8], uint32_t m, bool ok, int lane, uint32_t& word) {
+    const uint32_t sb = scale_block<kE2M1>(f, m);
+    word = ok ? sb << (8 * ((lane >> 2) & 3)) : 0u;
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    return sb == 255u ? 0u : pack_e2m1x8(f);
+}
+
 // ---- 4-bit matrices: where the scale bytes lie ----
 // The tensor cores read the scales of 128 rows x 4 blocks (128 columns) as one 512-byte tile: byte
 // (row % 32) * 16 + (row % 128 / 32) * 4 + block % 4, copied to tensor memory as it is. A matrix keeps them in that

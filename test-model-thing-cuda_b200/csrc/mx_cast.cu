@@ -37,22 +37,10 @@ __device__ __forceinline__ Vec8<F32> load8(const void* X, size_t at) {
     }
     return v;
 }
-// the 8 values and the fp32 bits of the largest magnitude among them
 template <bool F32>
-__device__ __forceinline__ uint32_t spread8(const Vec8<F32>& v, float (&f)[8]) {
-    if constexpr (F32) {
-        const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { f[i] = __uint_as_float(w[i]); m = max(m, w[i] & 0x7fffffffu); }
-        return m;
-    } else {
-        const uint32_t w[4] = {v.a.x, v.a.y, v.a.z, v.a.w};
-        uint32_t m = 0;                                       // two 16-bit maxima: magnitudes of bf16 order like their bits
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); m = __vmaxu2(m, w[i] & 0x7fff7fffu); }
-        return max(m >> 16, m & 0xffffu) << 16;
-    }
+__device__ __forceinline__ uint32_t spread(const Vec8<F32>& v, float (&f)[8]) {
+    if constexpr (F32) return spread8(v.a, v.b, f);
+    else return spread8(v.a, f);
 }
 
 template <int FMT, bool F32, int U>
@@ -62,7 +50,6 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __res
     if (early) pdl_begin();
     const int lane = threadIdx.x & 31;
     const unsigned c0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * U;
-    const unsigned full = 0xffffffffu;
     size_t at[U]; unsigned row[U]; int col[U]; bool ok[U];
     Vec8<F32> v[U];
 #pragma unroll
@@ -81,21 +68,12 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const void* __res
     for (int u = 0; u < U; ++u) {
         if (FMT != kE2M1 && c0 + u >= chunks) break;          // whole warps leave together
         float f[8];
-        uint32_t m = spread8<F32>(v[u], f);
-        m = max(m, __shfl_xor_sync(full, m, 1));
-        m = max(m, __shfl_xor_sync(full, m, 2));
-        const uint32_t sb = scale_byte<FMT>(m);
-        const float inv = inv_scale(sb);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= inv;
+        const uint32_t m = spread<F32>(v[u], f);
         if constexpr (FMT == kE2M1) {
-            uint32_t q = pack_e2m1x8(f);
-            if (sb == 255u) q = 0;
+            const uint32_t q = quantize8_e2m1(f, m, ok[u], lane, word[u]);
             if (ok[u]) *reinterpret_cast<uint32_t*>(codes + at[u] / 2) = q;
-            uint32_t w = ok[u] ? sb << (8 * ((lane >> 2) & 3)) : 0u;      // the word of 4 blocks; blocks past the last column are 0
-            w |= __shfl_xor_sync(full, w, 4);
-            word[u] = w | __shfl_xor_sync(full, w, 8);
         } else {
+            const uint32_t sb = scale_block<FMT>(f, m);
             uint32_t lo = pack_f8x4<FMT>(f[0], f[1], f[2], f[3]), hi = pack_f8x4<FMT>(f[4], f[5], f[6], f[7]);
             if (sb == 255u) { lo = 0; hi = 0; }
             if (ok[u]) {

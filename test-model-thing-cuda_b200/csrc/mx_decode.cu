@@ -34,9 +34,6 @@ constexpr uint32_t kSfACol = 2 * kRows, kSfWCol = kSfACol + 16, kTmemCols = 256;
 static_assert(kSfWCol + 8 * kMaxStages <= kTmemCols, "tensor memory");
 constexpr unsigned kFull = 0xffffffffu;
 
-__device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
 __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -50,15 +47,9 @@ __device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {       // the word at this offset of another block of the cluster
-    uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(addr, (uint32_t)rank)) : "memory");
     return v;
 }
 
@@ -89,27 +80,10 @@ struct Piece {
         uint32_t q = a.x, word = sw;
         if constexpr (SRC == kMxSrcBf16 || SRC == kMxSrcF32) {
             float f[8];
-            uint32_t m = 0;
-            if constexpr (SRC == kMxSrcF32) {
-                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) { f[j] = __uint_as_float(w[j]); m = max(m, w[j] & 0x7fffffffu); }
-            } else {
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { f[2 * j] = bf_lo(w[j]); f[2 * j + 1] = bf_hi(w[j]); m = __vmaxu2(m, w[j] & 0x7fff7fffu); }
-                m = max(m >> 16, m & 0xffffu) << 16;
-            }
-            m = max(m, __shfl_xor_sync(kFull, m, 1));
-            m = max(m, __shfl_xor_sync(kFull, m, 2));
-            const uint32_t sb = scale_byte<kE2M1>(m);
-            const float inv = inv_scale(sb);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] *= inv;
-            q = sb == 255u ? 0u : pack_e2m1x8(f);
-            word = sb << (8 * ((lane >> 2) & 3));
-            word |= __shfl_xor_sync(kFull, word, 4);
-            word |= __shfl_xor_sync(kFull, word, 8);
+            uint32_t m;
+            if constexpr (SRC == kMxSrcF32) m = spread8(a, b, f);
+            else m = spread8(a, f);
+            q = quantize8_e2m1(f, m, true, lane, word);
         }
         const uint32_t stage = act + kb * kStageA;
         st_shared4(stage + r * 128 + ((((uint32_t)lane >> 2) ^ (uint32_t)(r & 7)) << 4) + (lane & 3) * 4, q);

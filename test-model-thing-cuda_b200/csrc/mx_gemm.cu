@@ -32,24 +32,19 @@ constexpr int kBP = 128;                 // rows of a tile on the P side
 constexpr int kThreads = 352;
 constexpr int kOutBox = 32 * 128;        // staged outputs of a warp: its 32 rows x 128 bytes
 
-template <int BN> struct Shape {
-    static constexpr int kQBands = (BN + 127) / 128;                     // 128-row bands of scale tiles on the Q side
-    static constexpr int kCodesP = kBP * 128, kCodesQ = BN * 128;
-    static constexpr int kSfP = 2 * kScaleTile, kSfQ = 2 * kScaleTile * kQBands;
-    static constexpr int kStageBytes = kCodesP + kCodesQ + kSfP + kSfQ;
-    static constexpr int kStages = (220 * 1024 - 8 * kOutBox) / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + 8 * kOutBox + 1024;
-    static constexpr uint32_t kSfCol = 2 * BN;                           // scale columns follow the two accumulators
-    static constexpr uint32_t kCols = 2 * BN + 8 + 8 * kQBands <= 128 ? 128 : 2 * BN + 8 + 8 * kQBands <= 256 ? 256 : 512;
-    static_assert(2 * BN + 8 + 8 * kQBands <= 512, "tensor memory has 512 columns");
-};
+constexpr int kBQ = 128;                 // and on the Q side
+constexpr int kCodesP = kBP * 128, kCodesQ = kBQ * 128;
+constexpr int kSf = 2 * kScaleTile;      // scale tiles of either side
+constexpr int kStageBytes = kCodesP + kCodesQ + 2 * kSf;
+constexpr int kStages = (220 * 1024 - 8 * kOutBox) / kStageBytes;
+constexpr int kSmem = kStages * kStageBytes + 8 * kOutBox + 1024;
+constexpr uint32_t kSfCol = 2 * kBQ;     // scale columns follow the two accumulators
+constexpr uint32_t kTmemCols = 512;
+static_assert(kSfCol + 16 <= kTmemCols, "tensor memory");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 __device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t dp, uint64_t dq, uint32_t idesc, uint32_t sfp, uint32_t sfq, uint32_t accumulate) {
     asm volatile(
@@ -125,40 +120,38 @@ __device__ __forceinline__ void drain_tile(const MxGemm& p, const Tile& ti, uint
     }
 }
 
-template <int BN, int EPI>
+template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_constant__ MxGemm p) {
-    using S = Shape<BN>;
-    constexpr int TA = kBP, TW = BN;       // activation / weight rows of a tile
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full_bar[S::kStages], empty_bar[S::kStages], tfull_bar[2], tempty_bar[2];
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], tfull_bar[2], tempty_bar[2];
     __shared__ Groups groups;
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t codes_p = base, codes_q = base + S::kStages * S::kCodesP, sf_p = codes_q + S::kStages * S::kCodesQ, sf_q = sf_p + S::kStages * S::kSfP;
+    const uint32_t codes_p = base, codes_q = base + kStages * kCodesP, sf_p = codes_q + kStages * kCodesQ, sf_q = sf_p + kStages * kSf;
     volatile int* abort_flag = &abort_s;
 
     if (threadIdx.x == 0) {
         abort_s = 0;
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&empty_bar[s]), 1); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&empty_bar[s]), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(S::kCols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         pdl_begin();                         // not before: the next kernel could take the tensor memory this one is about to ask for
     }
     pdl_wait();
-    load_groups<TA>(p, groups);
+    load_groups<kBP>(p, groups);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-    const int w_tiles = ceil_div(p.n, TW);
+    const int w_tiles = ceil_div(p.n, kBQ);
     const int nkb = ceil_div(p.k, kKB);
     const int tiles_k = scale_tiles_k(p.k);
 
@@ -171,12 +164,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
             bool ok = true;
             for (int t = blockIdx.x; ok; t += gridDim.x) {
                 Tile ti;
-                if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+                if (!get_tile<kBP, kBQ>(p, groups, t, w_tiles, ti)) break;
                 const CUtensorMap* map;
                 const uint8_t* sc;
                 int row;
-                long band;                                     // first 128-row band of scale tiles
-                int bands = 1;
                 if (is_p) {
                     map = &p.act; sc = p.act_scales; row = ti.row0;
                 } else {
@@ -185,25 +176,23 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
                     row = ti.w0;
                     if (p.w_maps) tensormap_acquire(map);
                 }
-                band = row >> 7;
-                if (!is_p) bands = min(S::kQBands, (p.n - row + 127) / 128);
+                const size_t band = (size_t)(row >> 7) * tiles_k;      // first scale tile of the tile's 128 rows
                 for (int kb = 0; kb < nkb; ++kb) {
                     ok = mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, p.status);
                     if (!ok) break;
                     const uint32_t fb = smem_u32(&full_bar[s]);
                     const uint32_t sf_bytes = (uint32_t)min(2, tiles_k - 2 * kb) * kScaleTile;
-                    mbar_expect_tx(fb, (is_p ? S::kCodesP : S::kCodesQ) + bands * sf_bytes);
-                    tma_load_2d(is_p ? codes_p + s * S::kCodesP : codes_q + s * S::kCodesQ, map, fb, kb * 128, row);
-                    const uint32_t sf = is_p ? sf_p + s * S::kSfP : sf_q + s * S::kSfQ;
-                    for (int b = 0; b < bands; ++b)
-                        bulk_load(sf + b * 2 * kScaleTile, sc + ((size_t)(band + b) * tiles_k + 2 * kb) * kScaleTile, sf_bytes, fb);
+                    static_assert(kCodesP == kCodesQ, "one box size for both operands");
+                    mbar_expect_tx(fb, kCodesP + sf_bytes);
+                    tma_load_2d((is_p ? codes_p : codes_q) + s * kCodesP, map, fb, kb * 128, row);
+                    bulk_load((is_p ? sf_p : sf_q) + s * kSf, sc + (band + 2 * kb) * kScaleTile, sf_bytes, fb);
                     issued |= 1u << s;
                     last_parity = (last_parity & ~(1u << s)) | (ph << s);
-                    if (++s == S::kStages) { s = 0; ph ^= 1; }
+                    if (++s == kStages) { s = 0; ph ^= 1; }
                 }
             }
             if (!ok)       // aborting: wait (bounded) until the copies already issued have landed
-                for (int q = 0; q < S::kStages; ++q) {
+                for (int q = 0; q < kStages; ++q) {
                     if (!(issued >> q & 1)) continue;
                     const long long t0 = clock64();
                     while (!mbar_try_wait(smem_u32(&full_bar[q]), (last_parity >> q) & 1) && clock64() - t0 < kWaitCycles) {}
@@ -212,44 +201,42 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
         __syncwarp();
     } else if (warp == 1) {
         // ---------------- MMA issuer: the whole warp runs the loop, one elected lane issues ----------------
-        const uint32_t sfp_t = tmem_base + S::kSfCol, sfq_t = sfp_t + 8;
-        const uint32_t idesc0 = mxf4_idesc(kBP, BN);
+        const uint32_t sfp_t = tmem_base + kSfCol, sfq_t = sfp_t + 8;
+        const uint32_t idesc0 = mxf4_idesc(kBP, kBQ);
         int s = 0; uint32_t ph = 0;
         int acc = 0; uint32_t acc_ph = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok; t += gridDim.x) {
             Tile ti;
-            if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+            if (!get_tile<kBP, kBQ>(p, groups, t, w_tiles, ti)) break;
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tempty_bar[acc]), acc_ph ^ 1, abort_flag, p.status));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d_tmem = tmem_base + acc * BN;
+            const uint32_t d_tmem = tmem_base + acc * kBQ;
             for (int kb = 0; kb < nkb; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, p.status));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint64_t dp = make_desc(codes_p + s * S::kCodesP, false, 0), dq = make_desc(codes_q + s * S::kCodesQ, false, 0);
+                    const uint64_t dp = make_desc(codes_p + s * kCodesP, false, 0), dq = make_desc(codes_q + s * kCodesQ, false, 0);
                     const int steps = min(4, (p.k - kb * kKB) / 64);
 #pragma unroll
                     for (int a = 0; a < 2; ++a) {
                         if (2 * a < steps) {
-                            scale_copy(sfp_t + a * 4, scale_desc(sf_p + s * S::kSfP + a * kScaleTile));
-#pragma unroll
-                            for (int b = 0; b < S::kQBands; ++b)
-                                scale_copy(sfq_t + a * 4 * S::kQBands + b * 4, scale_desc(sf_q + s * S::kSfQ + b * 2 * kScaleTile + a * kScaleTile));
+                            scale_copy(sfp_t + a * 4, scale_desc(sf_p + s * kSf + a * kScaleTile));
+                            scale_copy(sfq_t + a * 4, scale_desc(sf_q + s * kSf + a * kScaleTile));
                         }
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (j < steps) {
                             mma_mxf4(d_tmem, dp + (uint64_t)(j * 2), dq + (uint64_t)(j * 2), idesc0 | mxf4_ids((j & 1) * 2), sfp_t + (j >> 1) * 4,
-                                     sfq_t + (j >> 1) * 4 * S::kQBands, (kb | j) != 0);
+                                     sfq_t + (j >> 1) * 4, (kb | j) != 0);
                         }
                     tc_commit(smem_u32(&empty_bar[s]));
                 }
                 __syncwarp();
-                if (++s == S::kStages) { s = 0; ph ^= 1; }
+                if (++s == kStages) { s = 0; ph ^= 1; }
             }
             if (!ok) break;
             if (elect_one()) tc_commit(smem_u32(&tfull_bar[acc]));
@@ -260,14 +247,14 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     } else {
         // ---------------- epilogue ----------------
         const int quarter = warp & 3, group = (warp - 2) >> 2;
-        const uint32_t buf = sf_q + S::kStages * S::kSfQ + (uint32_t)(warp - 2) * kOutBox;
+        const uint32_t buf = sf_q + kStages * kSf + (uint32_t)(warp - 2) * kOutBox;
         int acc = 0; uint32_t acc_ph = 0;
         for (int t = blockIdx.x;; t += gridDim.x) {
             Tile ti;
-            if (!get_tile<TA, TW>(p, groups, t, w_tiles, ti)) break;
+            if (!get_tile<kBP, kBQ>(p, groups, t, w_tiles, ti)) break;
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[acc]), acc_ph, abort_flag, p.status))) break;
             tc_fence_after();
-            const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
+            const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kBQ);
             drain_tile<EPI>(p, ti, tm, quarter, group, buf, smem_u32(&tempty_bar[acc]), lane);
             if (++acc == 2) { acc = 0; acc_ph ^= 1; }
         }
@@ -276,26 +263,15 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const __grid_const
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kCols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
     }
 }
 
-template <int BN, int EPI>
+template <int EPI>
 cudaError_t launch_t(const MxGemm& p, int grid, cudaStream_t stream) {
-    constexpr int smem = Shape<BN>::kSmem;
-    const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(mx_gemm_kernel<BN, EPI>, dim3(grid), dim3(kThreads), smem, stream, p);
-}
-template <int BN>
-cudaError_t launch_epi(const MxGemm& p, int grid, cudaStream_t stream) {
-    switch (p.epi) {
-        case kMxBf16: return launch_t<BN, kMxBf16>(p, grid, stream);
-        case kMxF32: return launch_t<BN, kMxF32>(p, grid, stream);
-        case kMxUp: return launch_t<BN, kMxUp>(p, grid, stream);
-        case kMxDown: return launch_t<BN, kMxDown>(p, grid, stream);
-        default: return cudaErrorInvalidValue;
-    }
+    return launch_pdl(mx_gemm_kernel<EPI>, dim3(grid), dim3(kThreads), kSmem, stream, p);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -360,7 +336,13 @@ void mx_make_out_map(CUtensorMap* m, void* out, uint64_t rows, int n, bool f32) 
 
 cudaError_t launch_mx_gemm(const MxGemm& p, int num_sms, cudaStream_t stream) {
     if (p.form == kMxPair) return launch_mx_gemm_2cta(p, num_sms, stream);
-    return launch_epi<128>(p, num_sms, stream);
+    switch (p.epi) {
+        case kMxBf16: return launch_t<kMxBf16>(p, num_sms, stream);
+        case kMxF32: return launch_t<kMxF32>(p, num_sms, stream);
+        case kMxUp: return launch_t<kMxUp>(p, num_sms, stream);
+        case kMxDown: return launch_t<kMxDown>(p, num_sms, stream);
+        default: return cudaErrorInvalidValue;
+    }
 }
 
 }  // namespace tmt

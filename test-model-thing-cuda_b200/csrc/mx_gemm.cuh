@@ -21,6 +21,19 @@ __device__ __forceinline__ uint32_t mxf4_ids(uint32_t id) { return (id << 4) | (
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
 }
+// a scale tile into 4 columns of tensor memory: 32 lanes x 16 bytes, repeated for the four lane quarters
+__device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {      // this address in another CTA of the cluster
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 struct Groups {                          // in shared memory: the experts' groups and their tiles on the activation side
     int first[kMaxExperts + 1];          // first activation tile of each group
     int poff[kMaxExperts], count[kMaxExperts];

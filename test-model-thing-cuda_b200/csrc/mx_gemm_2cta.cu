@@ -51,15 +51,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // No memory is handed over with these arrivals, only tensor memory (ordered by the tcgen05 fences), so they carry no release at
 // cluster scope: with one, a warp waited some 1100 clocks for its earlier writes before the next tile's MMAs could start.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {

@@ -63,11 +63,11 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
             slot = table[e] + b.rank[t * d.K + lane];
             if (slot < 0 || slot >= d.cap) { report(b.status, kErrSlotRange); slot = -1; }
             else {
-                b.slot_of[t * d.K + lane] = slot;
                 b.slotw[slot] = b.w[t * d.K + lane];
                 b.tok_of_slot[slot] = (int)t;
             }
         }
+        b.slot_of[t * d.K + lane] = slot;        // -1: the combine leaves the row out
     }
     int slots[kMaxTopk];
 #pragma unroll
@@ -79,22 +79,9 @@ __global__ void __launch_bounds__(kDispatchWarps * 32) mx_dispatch_kernel(const 
         const bool ok = col < d.D;
         uint4 x = make_uint4(0, 0, 0, 0);
         if (ok) x = ldg16(src + col);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         float f[8];
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); m = __vmaxu2(m, w[i] & 0x7fff7fffu); }
-        m = max(m >> 16, m & 0xffffu) << 16;
-        m = max(m, __shfl_xor_sync(full, m, 1));
-        m = max(m, __shfl_xor_sync(full, m, 2));
-        const uint32_t sb = scale_byte<kE2M1>(m);
-        const float inv = inv_scale(sb);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= inv;
-        const uint32_t q = sb == 255u ? 0u : pack_e2m1x8(f);
-        uint32_t word = ok ? sb << (8 * ((lane >> 2) & 3)) : 0u;
-        word |= __shfl_xor_sync(full, word, 4);
-        word |= __shfl_xor_sync(full, word, 8);
+        uint32_t word;
+        const uint32_t m = spread8(x, f), q = quantize8_e2m1(f, m, ok, lane, word);
         if (ok) {
 #pragma unroll
             for (int j = 0; j < kMaxTopk; ++j)
