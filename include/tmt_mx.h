@@ -19,7 +19,8 @@
  * (what cudaMalloc returns is), nothing allocates, nothing synchronises, nothing calls exit(). Work is queued on `stream`
  * of the current device; a tensor that lies on another device or in host memory is refused. Outputs and workspaces overlap
  * neither each other nor an input.
- * Calls without a handle may run side by side on several streams (they share no state), and may be captured into a graph.
+ * Calls without a handle may run side by side on several streams (they share no state but the word of tmt_moe_mxfp4_status),
+ * and may be captured into a graph.
  * rows = 0 is allowed where no handle is involved and does nothing.
  *
  * Kernels of these operators may be scheduled while the one before them on the stream is still running (programmatic launch;

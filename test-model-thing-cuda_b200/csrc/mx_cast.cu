@@ -3,7 +3,9 @@
 // A warp takes 256 neighbouring elements of a row, 8 per lane, so that a block of 32 is 4 lanes: one 16-byte load per lane
 // (two for fp32), the block's largest magnitude by two shuffles, one store of 4 (e2m1) or 8 bytes (e4m3, e5m2) per lane. Every
 // byte moves once; bound by HBM. In 4 bits a warp takes the same 256 columns of the rows r, r + 32, r + 64 and r + 96 of a band of 128,
-// whose scale words are neighbours in the scale tile (single words, one row a warp, took 150 us instead of 114 at 131072 x 2048). Several such chunks are in flight per warp where there are enough of them (U).
+// whose scale words are neighbours in the scale tile (single words, one row a warp, took 150 us instead of 114 at 131072 x 2048). Several
+// such chunks are in flight per warp where there are enough of them (U). Rows below 256 columns leave lanes idle: 131072 x 64 takes 18 us
+// in either direction and format, beside a floor of 3 to 4, as 131072 x 256 does (20 | 13 to 16).
 // `early`: lets the next kernel of the stream be scheduled at once (launch_pdl.cuh). Only where that kernel is known to wait
 // before it reads anything: the product of a dense layer, whose barriers and tensor memory are then ready when this kernel ends.
 #include <cuda_runtime.h>

@@ -402,9 +402,9 @@ cudaError_t launch_dense(const MxDecode& p, cudaStream_t stream) {
 
 // A block alone takes k in turn, about 1.6 us per 1024 of it: from 2048 on a cluster shares it, as far as there are SMs. 1 row, us:
 //     n x k        alone  shared               n x k        alone  shared
-//     2048 x 2048    6.0     5.7               4096 x 4096    9.9     6.5
-//     1024 x 4096    9.8     5.7               1024 x 8192   15.8     6.4
-// Below 2048 a block alone is done sooner than any cluster was (1024 x 1024: 4.2): it starts early, which clusters go without.
+//     2048 x 2048    6.3     5.6               4096 x 4096   10.0     7.3
+//     1024 x 4096   10.0     5.6               1024 x 8192   16.9     6.5
+// Below 2048 a block alone is done sooner than any cluster was (1024 x 1024: 4.4): it starts early, which clusters go without.
 int mx_decode_split(int n, int k, int num_sms) {
     const int tiles = ceil_div(n, 128), nkb = ceil_div(k, kKB);
     int split = 1;
@@ -414,12 +414,12 @@ int mx_decode_split(int n, int k, int num_sms) {
 
 // Every block brings all rows in for itself, 0.03 us per row and 256 of its share of k, where quantising once and 128 x 128 tiles
 // cost the same for 1 row as for 128. Dense layers, us, few rows (1, 8, 16, 24, 32) | tiles:
-//      320 -> 4096   3.9   4.1   4.6   5.3   5.8 |  4.9         4096 -> 1024   5.7   5.9   6.5   7.1   7.6 |  9.7
-//     1024 -> 1024   4.3   4.9   6.0   7.1   8.0 |  5.7         4096 -> 4096   6.4   7.1   8.2   9.4  10.4 |  9.8
-//     2048 -> 2048   5.7   5.9   6.6   7.3   7.8 |  7.1         8192 -> 1024   6.4   7.0   8.1   9.1  10.1 | 14.8
+//      320 -> 4096   3.7   3.9   4.4   5.0   5.5 |  4.9         4096 -> 1024   5.6   5.8   6.4   7.0   7.5 |  9.9
+//     1024 -> 1024   4.4   5.0   5.9   6.9   7.9 |  5.4         4096 -> 4096   7.3   7.4   8.5   9.7  10.6 | 10.4
+//     2048 -> 2048   5.6   5.8   6.4   7.1   7.7 |  7.3         8192 -> 1024   6.5   6.8   7.9   8.9   9.9 | 15.2
 // and of codes, where only a k long enough to be shared pays:
-//     1024 -> 1024   4.4   5.0   5.6   6.3   7.0 |  4.0         4096 -> 4096   6.6   7.0   7.8   8.6   9.3 |  8.3
-//     2048 -> 2048   5.7   6.0   6.5   7.1   7.4 |  5.4         8192 -> 1024   6.4   6.8   7.6   8.3   9.0 | 13.2
+//     1024 -> 1024   6.2   6.7   7.5   8.3   9.2 |  3.8         4096 -> 4096   7.4   7.5   7.9   8.6   9.3 |  8.7
+//     2048 -> 2048   5.6   5.9   6.4   6.9   7.3 |  5.8         8192 -> 1024   6.6   6.8   7.5   8.2   8.9 | 13.5
 bool mx_decode_dense(long rows, int k, int split, bool codes) {
     if (k > kMxDecodeMaxK || rows > kMxDecodeRows) return false;
     const long nkb = ceil_div(k, kKB), work = rows * ((nkb + split - 1) / split);
@@ -428,8 +428,8 @@ bool mx_decode_dense(long rows, int k, int split, bool codes) {
 }
 
 // Experts, us for the whole pass, this kernel | scan, dispatch and tiles, by rows per expert:
-//     16 experts 1024 -> 2048:   2 rows 26.6 | 33.8     8 rows 29.8 | 34.2    16 rows 41.6 | 38.4
-//      4 experts  512 -> 1024:   2 rows 21.2 | 25.5     8 rows 22.1 | 26.4    32 rows 32.1 | 26.3
+//     16 experts 1024 -> 2048:   2 rows 24.3 | 31.5     8 rows 26.5 | 32.0    16 rows 36.5 | 36.1    32 rows 53 | 37
+//      4 experts  512 -> 1024:   2 rows 18.1 | 23.4     8 rows 20.0 | 23.2    16 rows 21.9 | 23.6    32 rows 30 | 23
 bool mx_decode_grouped(long rows, int groups, int k) {
     const long nkb = ceil_div(k, kKB);
     return rows <= kMxDecodeMaxAsg && k <= kMxDecodeMaxK && rows <= 20L * groups && rows * nkb <= 80L * groups;

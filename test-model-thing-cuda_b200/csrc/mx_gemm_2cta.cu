@@ -3,7 +3,7 @@
 //
 // Why a pair. A 4-bit MMA consumes operand bytes at the rate of a bf16 one: a 128 x 128 tile of one CTA needs 128 bytes per
 // clock and SM from L2, a 256 x 256 tile of a pair 64 (each CTA stages its 128 activation rows and half of the weight rows),
-// where L2 gives about 72 (measured for the bf16 kernels). Scales add 6 bytes per clock: a CTA stages the tiles of its own
+// where L2 gives about 72 (as measured for the bf16 pair kernel). Scales add 6 bytes per clock: a CTA stages the tiles of its own
 // 128 activation rows and of all 256 weight rows, because each CTA's tensor memory holds the scales of what it multiplies.
 //
 // Shared memory is the next bound: an MMA of 256 columns reads 4 KB of A and 4 KB of its B half per 128 clocks in each CTA, and
@@ -20,7 +20,8 @@
 // 200 clocks). An epilogue thread owns a row: it loads 64 columns, hands them back, and works from registers; outputs are staged
 // in shared memory and written by TMA stores.
 // Measured (1 TF/s = 10^12 FLOP/s; operands of random codes): 16384 x 8192 -> 8192 5350 TF/s, held by the power limit at 1.3 to 1.4 GHz (7530 TF/s
-// on zeros, at 1.965 GHz: 640 clocks per k block of 512 ideal); 65536 x 2048 -> 2048 118 us = 4660 TF/s; 16384 x 1024 -> 4096 36 us = 3800 TF/s,
+// on zeros, at 1.965 GHz: 640 clocks per k block of 512 ideal); 65536 x 2048 -> 2048 118 to 135 us = 4070 to 4660 TF/s; 16384 x 1024 -> 4096 36 to 42 us = 3300 to 3800 TF/s
+// (the longer times with other products right before and after),
 // 4000 clocks per tile of 2048 ideal: some 500 between the last product of a tile and the first of the next, the rest waits
 // for operands while the outputs (64 KB a tile and CTA) leave through the same L2 (without the stores: 33 us).
 // Waits are bounded as in the bf16 kernels; both CTAs always reach the closing cluster barrier before tensor memory is freed.

@@ -40,7 +40,8 @@ __device__ __forceinline__ float butterfly(float v) {
 // read of X) and the next row is fetched before the current one is reduced.
 // FMT: mx::kE4M3 / mx::kE5M2 leaves an 8-bit checkpoint of the row as well (a block of 32 is the vectors of 4 neighbouring
 // lanes): one byte more per element written, and no second read of X. 0: none.
-// Bound: HBM; 131072 x 2048 takes 196 us without a checkpoint (5.5 TB/s) and 251 with one (5.4), 131072 x 1024 100 and 126. Several rows a
+// Bound: HBM; 131072 x 2048 takes 196 us without a checkpoint (5.5 TB/s) and 251 to 279 with one (4.8 to 5.4), 131072 x 1024 100 and 124; rows
+// below 256 columns leave lanes idle: 131072 x 32 44, x 64 45, x 128 45, x 256 51 with one. Several rows a
 // warp without the fetch ahead: 175 and 246 at 2048, but 10.6 and 17.0 instead of 8.8 and 11.6 at 8000 x 1024; the codes
 // packed in the first pass, next to the sums: 291 at 2048 (registers).
 template <int NV, int FMT>

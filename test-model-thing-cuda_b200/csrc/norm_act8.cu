@@ -13,7 +13,10 @@
 // sums instead of 40) and one barrier. Rows travel through a ring of P rows in shared memory filled by cp.async; every thread
 // copies exactly the pieces it will read itself, so the ring needs no barrier, and its depth costs no registers. The products run
 // on the packed fp32 pair instructions.
-// Measured at 131072 x 2048 (e4m3): 270 us = 5.0 TB/s, 0.77 of the copy rate; bound by issue slots (70 % busy). Two rows a turn and
+// Measured at 131072 x 2048 (e4m3): 272 to 285 us = 4.9 TB/s, 0.75 of the copy rate; bound by latency at 16 warps an SM (128 registers a
+// thread): issue slots are 57 % busy, DRAM 55 to 75 %. Other widths, 131072 rows, us beside the floor: 32 columns 68 | 3, 64: 48 | 7, 128: 46 | 13,
+// 256: 53 | 26 (these by the column-sum kernel, which has 2 * dim / 32 blocks for the sums of up to 16384 teams), 1024: 142 | 105, 2080: 353 | 212;
+// 65536 x 4096 290 | 209, 32768 x 8192 290 | 209 (one block of up to 512 threads an SM, 36 bytes spilled). Two rows a turn and
 // three blocks an SM: 284-315; rows dealt round instead of in ranges: 380; two vectors a thread and four blocks: 375; the
 // row fetched ahead into registers instead of the ring: 343-365.
 // The column sums of the teams are added by a second kernel in a fixed order: results do not depend on timing.
