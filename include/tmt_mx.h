@@ -74,7 +74,8 @@ size_t tmt_moe_linear_mxfp4_work_bytes(long long rows, int cols);
 int tmt_moe_linear_mxfp4(const void* X, int x_dtype, int rows, const tmt_mxfp4_weight* W, void* Y, int y_dtype, void* work,
                          size_t work_bytes, int* status, void* stream);
 /* The first code that a product without a status word of its own has recorded on the current device since the last call of this
- * function, 0 when there is none; -1 on an error. Waits for the device, and clears the word. */
+ * function, 0 when there is none; -1 on an error. Waits for the device (so not while a stream is being captured), and clears
+ * the word. */
 int tmt_moe_mxfp4_status(void);
 /* Failure-detection self-test of that word: queues one block that waits on a barrier nothing arrives on, limit_cycles clock cycles
  * long, through the same bounded wait as the products. tmt_moe_mxfp4_status then gives 2. */
@@ -94,7 +95,8 @@ int tmt_moe_linear_mxfp4_form(int rows, int n, int k);
  * recorded with, whatever later calls are given. */
 int tmt_moe_forward_mxfp4(tmt_moe* h, const void* X, const void* Wrouter, const tmt_mxfp4_weight* Wup,
                           const tmt_mxfp4_weight* Wdown, void* Y, float beta, int tokens);
-/* Which kernel the up (product 0) and the down product (1) of a call with `tokens` tokens take; -1 for arguments out of range. */
+/* Which kernel the up (product 0) and the down product (1) of a call with `tokens` tokens take; -1 for arguments out of
+ * range and for a handle without this pass. */
 int tmt_moe_forward_mxfp4_form(const tmt_moe* h, int tokens, int product);
 /* 1 when the weights last handed to tmt_moe_forward_mxfp4 were recorded into a graph (which goes on reading them), else 0; -1 for a
  * null handle. */

@@ -454,6 +454,7 @@ int tmt_moe_linear_mxfp4_form(int rows, int n, int k) {
 int tmt_moe_forward_mxfp4_form(const tmt_moe* h, int tokens, int product) {
     if (!h) { set_error("null handle"); return -1; }
     if (tokens < 1 || tokens > h->d.tokens || product < 0 || product > 1) { set_error("tokens outside [1, desc.tokens], or product not 0 or 1"); return -1; }
+    if (h->d.hidden == 0 || h->d.training || h->d.ep_world > 1) { set_error("MXFP4 forward needs hidden > 0, training = 0 and a single rank"); return -1; }
     return product == 0 ? experts_form(h, tokens, h->d.hidden, h->d.dim) : experts_form(h, tokens, h->d.dim, h->d.hidden);
 }
 

@@ -35,6 +35,8 @@ def test_what_the_library_says_of_a_shape():
     for product, tokens in ((2, 4), (-1, 4), (0, 0), (0, 65)):
         with pytest.raises(M.MoeError):
             moe.forward_mxfp4_form(product, tokens)
+    with pytest.raises(M.MoeError, match="training"):
+        M.MoE(64, 64, 2, 1, hidden=64, training=True).forward_mxfp4_form(0)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
